@@ -383,6 +383,119 @@ int pmoe_block_forward_noalloc(const uint16_t* x, int T, int H, int E, int K, in
 /* Size in bytes of the fixed scratch array of pmoe_block_forward_noalloc. */
 size_t pmoe_noalloc_scratch_bytes(void);
 
+/* ---- the attention half: rotary positions, paged cache, attention ------------
+ * What stands beside the MoE half of a decoder layer: the projections' q, k and v
+ * are turned by their positions, k and v are written to a paged cache, and
+ * attention reads it.  bf16 throughout; head dim D in {64, 128, 256}; page size in
+ * {16, 32, 64, 128}; Hq a multiple of Hkv, at most 128 query heads per key/value
+ * head (query head h reads key/value head h / (Hq / Hkv)).
+ *
+ * Cache: k_pages / v_pages are two views [n_pages][Hkv][page_size][D] (inner three
+ * dimensions contiguous; page strides in elements, multiples of 8).  Key j of
+ * sequence b lies in page page_table[b * table_stride + j / page_size], row
+ * j % page_size.  kv_lens[b] counts sequence b's keys, the call's new tokens
+ * included.  cu_q [B+1] int32: row t of a packed batch belongs to the sequence
+ * with cu_q[b] <= t < cu_q[b+1] (ascending) and is its token at index
+ * kv_lens[b] - (cu_q[b+1] - t).  Rows behind cu_q[B] belong to no sequence.
+ * A table entry outside [0, n_pages) names no page: nothing is read or written
+ * through it, and a row that sees such a key gets NaN.  Strides are in elements
+ * (multiples of 8; the innermost dimension is contiguous).  The reference runs
+ * this half through the HF module (Qwen3_5MoeAttention) and its slot-pool cache
+ * (engine/runtime/kv_cache.py:220); it has no operator of its own for any of it.
+ *
+ * Rotary positions and cache write.  For each row of q and k: the optional
+ * per-head RMSNorm (w_qnorm / w_knorm [D], NULL: none; x * rsqrt(mean x^2 + eps) *
+ * (1 + w)), then pair (i, i + rot/2), i < rot/2, turned by
+ * positions[axis(i) * pos_stride + t] * inv_freq[i], cos and sin scaled by mscale;
+ * dims >= rot pass through.  axis(i): the section that i falls into
+ * (interleaved 0), or i % axes where i < axes * sections[i % axes], else 0
+ * (interleaved 1).  sections: host array of `axes` (1..4) counts that add up to
+ * rot/2; rot a multiple of 16.  Angles are formed in 64 bits.  q_out [T][Hq][D] gets
+ * all T rows; k and v go to the cache rows of their tokens (rows of no sequence,
+ * and tokens without a page, are not written).  cu_q NULL: one token per
+ * sequence, T == B. */
+int pmoe_rope_append(const uint16_t* q, int64_t q_stride_t, int64_t q_stride_h,
+                     const uint16_t* k, int64_t k_stride_t, int64_t k_stride_h,
+                     const uint16_t* v, int64_t v_stride_t, int64_t v_stride_h, int T, int Hq,
+                     int Hkv, int D, const int64_t* positions, int64_t pos_stride, int axes,
+                     const int* sections, int interleaved, const float* inv_freq, int rot,
+                     const uint16_t* w_qnorm, const uint16_t* w_knorm, float eps, float mscale,
+                     uint16_t* k_pages, uint16_t* v_pages, int64_t k_page_stride,
+                     int64_t v_page_stride, int n_pages, int page_size,
+                     const int32_t* page_table, int64_t table_stride, int max_pages,
+                     const int32_t* kv_lens, const int32_t* cu_q, int B, uint16_t* q_out,
+                     void* stream);
+
+/* Attention of one new token per sequence: out[b][h] = sum_j softmax_j(scale
+ * q.k_j) v_j over the keys j that the token at p = kv_lens[b] - 1 sees: j <= p and,
+ * with window > 0, j > p - window or j < sinks.  A sequence without keys gets
+ * zeros.  out [B][Hq][D].  Deterministic.  workspace: pmoe_attn_decode_workspace
+ * bytes, its contents irrelevant before and after; calls that may overlap need
+ * workspaces of their own. */
+int pmoe_attn_decode_workspace(int B, int Hq, int Hkv, int D, size_t* bytes);
+int pmoe_attn_decode(const uint16_t* q, int64_t q_stride_t, int64_t q_stride_h, int B, int Hq,
+                     int Hkv, int D, const uint16_t* k_pages, const uint16_t* v_pages,
+                     int64_t k_page_stride, int64_t v_page_stride, int n_pages, int page_size,
+                     const int32_t* page_table, int64_t table_stride, int max_pages,
+                     const int32_t* kv_lens, float scale, int window, int sinks, uint16_t* out,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* The same for a packed batch of prompts or prompt chunks (cu_q): causal, with
+ * the cached keys before them, the same window and sinks.  out [T][Hq][D]; rows of no
+ * sequence, and rows at an index below zero, get zeros.  Deterministic. */
+int pmoe_attn_prefill(const uint16_t* q, int64_t q_stride_t, int64_t q_stride_h, int T, int Hq,
+                      int Hkv, int D, const uint16_t* k_pages, const uint16_t* v_pages,
+                      int64_t k_page_stride, int64_t v_page_stride, int n_pages, int page_size,
+                      const int32_t* page_table, int64_t table_stride, int max_pages,
+                      const int32_t* kv_lens, const int32_t* cu_q, int B, float scale,
+                      int window, int sinks, uint16_t* out, void* stream);
+
+/* ---- pages of the cache --------------------------------------------------------
+ * Device-side state of a pool of n_pages pages, `chunks` blocks of [page_size][D]
+ * bf16 each, contiguous ([n_pages][chunks][page_size][D]; chunks = layers * 2 * Hkv):
+ * refs [n_pages] int32 (sequences that hold the page, 0: free), tables [S] rows of
+ * max_pages int32 (-1: no page), lens [S] int32.  All four calls run in stream
+ * order without a host sync, can be captured, and are deterministic: free pages are
+ * handed out lowest number first, requests served in list order.  workspace:
+ * pmoe_pages_workspace bytes, contents irrelevant before and after.
+ *
+ * grow: sequence slots[i] gets add[i] more tokens and the pages they need.  ok[i] =
+ * 1, or 0 and nothing changed: a slot out of range, add < 0, a length beyond the
+ * table, a slot that an earlier request of the call names, or no pages left (the
+ * first request that does not fit ends the call's grants, apart from requests that
+ * are refused for another reason). */
+int pmoe_pages_workspace(int S, int n, int n_pages, size_t* bytes);
+int pmoe_pages_grow(int32_t* refs, int n_pages, int page_size, int32_t* tables,
+                    int64_t table_stride, int max_pages, int S, int32_t* lens,
+                    const int32_t* slots, const int32_t* add, int n, int32_t* ok,
+                    void* workspace, size_t workspace_bytes, void* stream);
+
+/* fork: empty sequence dst[i] becomes the first keep[i] tokens of src[i]: the full
+ * pages are shared (refs + 1), a partly filled last page is copied (its used rows) into
+ * a fresh one.  ok[i] = 1, or 0 and nothing changed: an index out of range, dst[i]
+ * not empty, named by an earlier request or the source of any request, keep[i] < 0
+ * or beyond the source's length, or no page left (as in grow). */
+int pmoe_pages_fork(uint16_t* pages, int n_pages, int chunks, int page_size, int D,
+                    int32_t* refs, int32_t* tables, int64_t table_stride, int max_pages, int S,
+                    int32_t* lens, const int32_t* src, const int32_t* dst, const int32_t* keep,
+                    int n, int32_t* ok, void* workspace, size_t workspace_bytes, void* stream);
+
+/* free: window 0: sequences slots[i] give up all their pages (refs - 1), their
+ * entries become -1 and their lengths 0.  window > 0: only the pages that no token
+ * from index lens - 1 on sees (wholly behind the window and the sinks); lengths stay.
+ * Slots out of range are skipped; one that is listed twice is freed once. */
+int pmoe_pages_free(int32_t* refs, int n_pages, int page_size, int32_t* tables,
+                    int64_t table_stride, int max_pages, int S, int32_t* lens,
+                    const int32_t* slots, int n, int window, int sinks, void* stream);
+
+/* compact: the live pages move to the front of the pool; tables and refs follow.
+ * live[0] = number of live pages; remap [n_pages] = a page's new number (-1: free).
+ * The k-th free page below live[0] receives the k-th live page above. */
+int pmoe_pages_compact(uint16_t* pages, int n_pages, int chunks, int page_size, int D,
+                       int32_t* refs, int32_t* tables, int64_t table_stride, int max_pages,
+                       int S, int32_t* live, int32_t* remap, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

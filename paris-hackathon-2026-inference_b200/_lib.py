@@ -17,6 +17,8 @@ LIB_PATH = os.path.join(_PKG, "libparis_moe.so")
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _SZ = ctypes.c_size_t
+_L = ctypes.c_int64
+_F = ctypes.c_float
 SIGNATURES = {
     "pmoe_status_string": (ctypes.c_char_p, [_I]),
     "pmoe_version": (ctypes.c_char_p, []),
@@ -74,6 +76,20 @@ SIGNATURES = {
     "pmoe_ipc_handle": (_I, [_P, ctypes.c_char_p]),
     "pmoe_ipc_open": (_I, [ctypes.c_char_p, ctypes.POINTER(_P)]),
     "pmoe_ipc_close": (_I, [_P]),
+    "pmoe_rope_append": (_I, [_P, _L, _L, _P, _L, _L, _P, _L, _L, _I, _I, _I, _I, _P, _L, _I,
+                              ctypes.POINTER(_I), _I, _P, _I, _P, _P, _F, _F, _P, _P, _L, _L,
+                              _I, _I, _P, _L, _I, _P, _P, _I, _P, _P]),
+    "pmoe_attn_decode_workspace": (_I, [_I, _I, _I, _I, ctypes.POINTER(_SZ)]),
+    "pmoe_attn_decode": (_I, [_P, _L, _L, _I, _I, _I, _I, _P, _P, _L, _L, _I, _I, _P, _L, _I,
+                              _P, _F, _I, _I, _P, _P, _SZ, _P]),
+    "pmoe_attn_prefill": (_I, [_P, _L, _L, _I, _I, _I, _I, _P, _P, _L, _L, _I, _I, _P, _L, _I,
+                               _P, _P, _I, _F, _I, _I, _P, _P]),
+    "pmoe_pages_workspace": (_I, [_I, _I, _I, ctypes.POINTER(_SZ)]),
+    "pmoe_pages_grow": (_I, [_P, _I, _I, _P, _L, _I, _I, _P, _P, _P, _I, _P, _P, _SZ, _P]),
+    "pmoe_pages_fork": (_I, [_P, _I, _I, _I, _I, _P, _P, _L, _I, _I, _P, _P, _P, _P, _I, _P,
+                             _P, _SZ, _P]),
+    "pmoe_pages_free": (_I, [_P, _I, _I, _P, _L, _I, _I, _P, _P, _I, _I, _I, _P]),
+    "pmoe_pages_compact": (_I, [_P, _I, _I, _I, _I, _P, _P, _L, _I, _I, _P, _P, _P, _SZ, _P]),
 }
 
 PMOE_ERR_PEER_TIMEOUT = -6

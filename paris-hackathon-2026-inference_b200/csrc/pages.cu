@@ -1,0 +1,314 @@
+// Page bookkeeping of the paged cache, all on the device and in stream order: grow, fork,
+// free and compact.  The state is refs[page] (sequences that hold the page; 0 = free), the
+// tables and the lengths; the free pages are those with refs 0, handed out lowest number
+// first, so the same calls give the same pages on every run.
+#include "paged.cuh"
+
+namespace pmoe {
+
+namespace {
+
+constexpr int kPlanThreads = 1024;
+constexpr int kPerThread = 4;
+
+// Inclusive scan of x over the block; *total gets the sum.
+__device__ __forceinline__ int block_scan(int x, int* s_warp, int* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();  // s_warp of the scan before has been read
+  if (lane == 31) s_warp[warp] = x;
+  __syncthreads();
+  int w = s_warp[lane];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, w, o);
+    if (lane >= o) w += y;
+  }
+  *total = __shfl_sync(0xffffffffu, w, 31);
+  const int before = __shfl_sync(0xffffffffu, w, warp == 0 ? 0 : warp - 1);
+  return x + (warp == 0 ? 0 : before);
+}
+
+// The first `want` free pages in ascending order into pick; returns how many there were.
+__device__ __forceinline__ int pick_free(const int32_t* refs, int n_pages, int want,
+                                         int32_t* pick, int* s_warp) {
+  int found = 0;
+  for (int p0 = 0; p0 < n_pages && found < want; p0 += kPlanThreads * kPerThread) {
+    const int p = p0 + threadIdx.x * kPerThread;
+    bool open[kPerThread];
+    int mine = 0, total;
+#pragma unroll
+    for (int k = 0; k < kPerThread; ++k) {
+      open[k] = p + k < n_pages && refs[p + k] == 0;
+      mine += open[k];
+    }
+    int at = found + block_scan(mine, s_warp, &total) - mine;
+#pragma unroll
+    for (int k = 0; k < kPerThread; ++k)
+      if (open[k]) {
+        if (at < want) pick[at] = p + k;
+        ++at;
+      }
+    found += total;
+  }
+  return min(found, want);
+}
+
+// mark[slot] = the first request that names the slot.
+__device__ __forceinline__ void mark_first(int32_t* mark, int S, const int32_t* slots, int n) {
+  for (int s = threadIdx.x; s < S; s += kPlanThreads) mark[s] = 0x7fffffff;
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += kPlanThreads)
+    if (slots[i] >= 0 && slots[i] < S) atomicMin(&mark[slots[i]], i);
+  __syncthreads();
+}
+
+__global__ void __launch_bounds__(kPlanThreads) pages_grow_kernel(
+    const Pool p, const int32_t* slots, const int32_t* add, int n, int32_t* ok, int32_t* ws) {
+  __shared__ int s_warp[32];
+  int32_t *mark = ws, *need = mark + p.S, *end = need + n, *pick = end + n;
+  const int tid = threadIdx.x, ps = 1 << p.page_shift;
+  mark_first(mark, p.S, slots, n);
+  int64_t carry = 0;
+  for (int i0 = 0; i0 < n; i0 += kPlanThreads) {
+    const int i = i0 + tid;
+    int want = -1;  // -1: refused
+    if (i < n) {
+      const int s = slots[i];
+      if (s >= 0 && s < p.S && mark[s] == i && add[i] >= 0) {
+        const int64_t old = p.lens[s], len = old + add[i];
+        if (old >= 0 && len <= int64_t(p.max_pages) << p.page_shift && len <= 0x7fffffff)
+          want = int(((len + ps - 1) >> p.page_shift) - ((old + ps - 1) >> p.page_shift));
+      }
+    }
+    int total;
+    const int64_t e = carry + block_scan(max(want, 0), s_warp, &total);
+    if (i < n) {
+      need[i] = want;
+      end[i] = int(min(e, int64_t(p.n_pages) + 1));  // beyond the pool: granted to nobody
+    }
+    carry += total;
+  }
+  __syncthreads();
+  const int found = pick_free(p.refs, p.n_pages, int(min(carry, int64_t(p.n_pages))), pick, s_warp);
+  __syncthreads();
+  const int lane = tid & 31;
+  for (int i = tid >> 5; i < n; i += kPlanThreads / 32) {
+    const int want = need[i], e = end[i], s = slots[i];
+    const bool yes = want >= 0 && e <= found;
+    if (yes) {
+      const int old = p.lens[s], first = int((int64_t(old) + ps - 1) >> p.page_shift);
+      for (int j = lane; j < want; j += 32) {
+        const int page = pick[e - want + j];
+        p.tables[s * p.table_stride + first + j] = page;
+        p.refs[page] = 1;
+      }
+      __syncwarp();
+      if (lane == 0) p.lens[s] = old + add[i];
+    }
+    if (lane == 0) ok[i] = yes;
+  }
+}
+
+// ws: mark[S], plan[n] (fresh page, -1: none needed, -2: refused), need[n], end[n], pick
+__global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(
+    const Pool p, const int32_t* src, const int32_t* dst, const int32_t* keep, int n,
+    int32_t* ok, int32_t* ws) {
+  __shared__ int s_warp[32];
+  int32_t *mark = ws, *plan = mark + p.S, *need = plan + n, *end = need + n, *pick = end + n;
+  const int tid = threadIdx.x, ps = 1 << p.page_shift;
+  mark_first(mark, p.S, dst, n);
+  int carry = 0;
+  for (int i0 = 0; i0 < n; i0 += kPlanThreads) {
+    const int i = i0 + tid;
+    int want = -1;
+    if (i < n) {
+      const int s = src[i], d = dst[i], k = keep[i];
+      // a target is empty, named once and nobody's source
+      if (s >= 0 && s < p.S && d >= 0 && d < p.S && mark[d] == i && mark[s] == 0x7fffffff &&
+          p.lens[d] == 0 && k >= 0 && k <= p.lens[s] &&
+          k <= int64_t(p.max_pages) << p.page_shift) {
+        want = 0;
+        if (k & (ps - 1)) {
+          const int t = p.tables[s * p.table_stride + (k >> p.page_shift)];
+          want = t >= 0 && t < p.n_pages;
+        }
+      }
+    }
+    int total;
+    const int e = carry + block_scan(max(want, 0), s_warp, &total);
+    if (i < n) need[i] = want, end[i] = e;
+    carry += total;
+  }
+  __syncthreads();
+  const int found = pick_free(p.refs, p.n_pages, min(carry, p.n_pages), pick, s_warp);
+  __syncthreads();
+  for (int i = tid; i < n; i += kPlanThreads) {
+    const bool yes = need[i] >= 0 && end[i] <= found;
+    ok[i] = yes;
+    plan[i] = !yes ? -2 : need[i] ? pick[end[i] - 1] : -1;
+  }
+}
+
+// gridDim = (n, parts): part 0 copies the table row, all parts copy the tail page.
+__global__ void __launch_bounds__(256) fork_copy_kernel(const Pool p, const int32_t* src,
+                                                        const int32_t* dst, const int32_t* keep,
+                                                        const int32_t* plan_ws) {
+  const int i = blockIdx.x, fresh = plan_ws[p.S + i];
+  if (fresh == -2) return;
+  const int k = keep[i], full = k >> p.page_shift, used = k & ((1 << p.page_shift) - 1);
+  const int32_t* from = p.tables + src[i] * p.table_stride;
+  if (blockIdx.y == 0) {
+    int32_t* to = p.tables + dst[i] * p.table_stride;
+    for (int j = threadIdx.x; j < full; j += blockDim.x) {
+      const int page = from[j];
+      to[j] = page;
+      if (page >= 0 && page < p.n_pages) atomicAdd(&p.refs[page], 1);
+    }
+    if (threadIdx.x == 0) {
+      if (fresh >= 0) {
+        to[full] = fresh;
+        p.refs[fresh] = 1;
+      }
+      p.lens[dst[i]] = k;
+    }
+  }
+  if (fresh < 0) return;
+  const size_t chunk = size_t(p.D) << p.page_shift;  // elements of one head's rows
+  const __nv_bfloat16* s0 = p.pages + size_t(from[full]) * p.chunks * chunk;
+  __nv_bfloat16* d0 = p.pages + size_t(fresh) * p.chunks * chunk;
+  const int vec = used * p.D / 8;  // 16-byte pieces of a chunk's used rows
+  for (int c = blockIdx.y; c < p.chunks; c += gridDim.y) {
+    const uint4* s = reinterpret_cast<const uint4*>(s0 + c * chunk);
+    uint4* d = reinterpret_cast<uint4*>(d0 + c * chunk);
+    for (int j = threadIdx.x; j < vec; j += blockDim.x) d[j] = s[j];
+  }
+}
+
+__global__ void __launch_bounds__(256) pages_free_kernel(const Pool p, const int32_t* slots,
+                                                         int window, int sinks) {
+  const int s = slots[blockIdx.x];
+  if (s < 0 || s >= p.S) return;
+  int lo = 0, hi = p.max_pages;
+  if (window > 0) {
+    const int ps = 1 << p.page_shift, len = p.lens[s];
+    lo = int((int64_t(sinks) + ps - 1) >> p.page_shift);
+    hi = min(hi, len > window ? (len - window) >> p.page_shift : 0);
+  }
+  int32_t* row = p.tables + s * p.table_stride;
+  for (int j = lo + threadIdx.x; j < hi; j += blockDim.x) {
+    if (row[j] < 0) continue;
+    // taken by one block alone where a slot is listed twice
+    const int page = atomicExch(&row[j], -1);
+    if (page >= 0 && page < p.n_pages) atomicSub(&p.refs[page], 1);
+  }
+  if (window == 0 && threadIdx.x == 0) p.lens[s] = 0;
+}
+
+// With n live pages, the k-th free page below n takes the k-th live page at or above it: a
+// packed pool after the fewest moves.  ws[0]: moves; ws[16 + k]: the k-th page that moves,
+// to remap[ws[16 + k]].
+__global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const Pool p, int32_t* live,
+                                                                    int32_t* remap, int32_t* ws) {
+  __shared__ int s_warp[32];
+  const int tid = threadIdx.x;
+  int32_t* movers = ws + 16;
+  int mine = 0, n_live;
+  for (int q = tid; q < p.n_pages; q += kPlanThreads) mine += p.refs[q] > 0;
+  block_scan(mine, s_warp, &n_live);
+  int moves = 0;
+  for (int q0 = 0; q0 < p.n_pages; q0 += kPlanThreads) {
+    const int q = q0 + tid;
+    const bool used = q < p.n_pages && p.refs[q] > 0;
+    const bool move = used && q >= n_live;
+    int total;
+    const int at = moves + block_scan(move, s_warp, &total) - move;
+    if (move) movers[at] = q;
+    if (q < p.n_pages) remap[q] = used ? q : -1;
+    moves += total;
+  }
+  __syncthreads();
+  int holes = 0;
+  for (int q0 = 0; q0 < n_live; q0 += kPlanThreads) {
+    const int q = q0 + tid;
+    const bool hole = q < n_live && p.refs[q] <= 0;
+    int total;
+    const int at = holes + block_scan(hole, s_warp, &total) - hole;
+    if (hole) remap[movers[at]] = q;
+    holes += total;
+  }
+  __syncthreads();
+  for (int k = tid; k < moves; k += kPlanThreads) {
+    const int from = movers[k], to = remap[from];
+    p.refs[to] = p.refs[from];
+    p.refs[from] = 0;
+  }
+  if (tid == 0) {
+    live[0] = n_live;
+    ws[0] = moves;
+  }
+}
+
+__global__ void __launch_bounds__(256) compact_move_kernel(const Pool p, const int32_t* remap,
+                                                           const int32_t* ws) {
+  const int moves = ws[0];
+  const int64_t entries = int64_t(p.S) * p.max_pages;
+  for (int64_t e = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; e < entries;
+       e += int64_t(gridDim.x) * blockDim.x) {
+    int32_t* at = p.tables + (e / p.max_pages) * p.table_stride + e % p.max_pages;
+    const int page = *at;
+    if (page >= 0 && page < p.n_pages) {
+      const int to = remap[page];
+      if (to >= 0 && to != page) *at = to;
+    }
+  }
+  const size_t page_vec = (size_t(p.chunks) * p.D << p.page_shift) / 8;
+  const size_t part = 2048;  // 16-byte pieces a block copies at a time
+  const size_t parts = (page_vec + part - 1) / part;
+  for (size_t w = blockIdx.x; w < parts * moves; w += gridDim.x) {
+    const int from = ws[16 + w / parts], to = remap[from];
+    const uint4* s = reinterpret_cast<const uint4*>(p.pages) + from * page_vec;
+    uint4* d = reinterpret_cast<uint4*>(p.pages) + to * page_vec;
+    const size_t j0 = (w % parts) * part, j1 = min(j0 + part, page_vec);
+    for (size_t j = j0 + threadIdx.x; j < j1; j += blockDim.x) d[j] = s[j];
+  }
+}
+
+}  // namespace
+
+cudaError_t launch_pages_grow(const Pool& p, const int32_t* slots, const int32_t* add, int n,
+                              int32_t* ok, int32_t* ws, cudaStream_t st) {
+  if (n == 0) return cudaSuccess;
+  pages_grow_kernel<<<1, kPlanThreads, 0, st>>>(p, slots, add, n, ok, ws);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_pages_fork(const Pool& p, const int32_t* src, const int32_t* dst,
+                              const int32_t* keep, int n, int32_t* ok, int32_t* ws,
+                              cudaStream_t st) {
+  if (n == 0) return cudaSuccess;
+  fork_plan_kernel<<<1, kPlanThreads, 0, st>>>(p, src, dst, keep, n, ok, ws);
+  const dim3 grid(n, p.chunks < 8 ? p.chunks : 8);
+  fork_copy_kernel<<<grid, 256, 0, st>>>(p, src, dst, keep, ws);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_pages_free(const Pool& p, const int32_t* slots, int n, int window, int sinks,
+                              cudaStream_t st) {
+  if (n == 0) return cudaSuccess;
+  pages_free_kernel<<<n, 256, 0, st>>>(p, slots, window, sinks);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_pages_compact(const Pool& p, int32_t* live, int32_t* remap, int32_t* ws,
+                                 cudaStream_t st) {
+  compact_plan_kernel<<<1, kPlanThreads, 0, st>>>(p, live, remap, ws);
+  compact_move_kernel<<<148 * 4, 256, 0, st>>>(p, remap, ws);
+  return cudaGetLastError();
+}
+
+}  // namespace pmoe

@@ -16,6 +16,7 @@
 #include <torch/library.h>
 
 #include <cstdint>
+#include <optional>
 #include <tuple>
 
 #include "paris_moe.h"
@@ -229,6 +230,316 @@ RouteOut moe_route_meta(const Tensor& x, const Tensor& w_router, const Tensor&, 
           at::empty({T * k}, i32), at::empty({T * k}, i32), at::empty({T}, f32)};
 }
 
+// ---- the attention half ------------------------------------------------------
+using OptTensor = std::optional<Tensor>;
+
+void check_int(const char* op, const char* name, const Tensor& t, at::ScalarType type, int dim,
+               const Tensor& x) {
+  TORCH_CHECK(t.is_cuda(), "paris_moe.", op, ": ", name, " must be a CUDA tensor");
+  TORCH_CHECK(t.device() == x.device(), "paris_moe.", op, ": ", name, " is on ", t.device(),
+              ", expected ", x.device());
+  TORCH_CHECK(t.scalar_type() == type, "paris_moe.", op, ": ", name, " must be ", type, ", got ",
+              t.scalar_type());
+  TORCH_CHECK(t.dim() == dim, "paris_moe.", op, ": ", name, " must have ", dim,
+              " dimensions, got ", t.dim());
+  TORCH_CHECK(t.numel() == 0 || t.size(dim - 1) <= 1 || t.stride(dim - 1) == 1, "paris_moe.", op,
+              ": ", name, "'s last dimension must be contiguous");
+}
+
+int to_int(const char* op, const char* name, int64_t v) {
+  TORCH_CHECK(v >= INT32_MIN && v <= INT32_MAX, "paris_moe.", op, ": ", name, " ", v,
+              " is beyond 32 bits");
+  return int(v);
+}
+
+// Element stride of a dimension; one of at most one entry is never stepped over.
+int64_t stride_of(const Tensor& t, int dim) { return t.size(dim) <= 1 ? 0 : t.stride(dim); }
+
+// Rows [T, heads, D]: any token and head stride, contiguous heads.
+void check_rows(const char* op, const char* name, const Tensor& t, const Tensor& x) {
+  TORCH_CHECK(t.is_cuda(), "paris_moe.", op, ": ", name, " must be a CUDA tensor");
+  TORCH_CHECK(t.device() == x.device(), "paris_moe.", op, ": ", name, " is on ", t.device(),
+              ", expected ", x.device());
+  TORCH_CHECK(t.scalar_type() == at::kBFloat16, "paris_moe.", op, ": ", name,
+              " must be bf16, got ", t.scalar_type());
+  TORCH_CHECK(t.dim() == 3, "paris_moe.", op, ": ", name, " must be [tokens, heads, D]");
+  TORCH_CHECK(t.size(2) <= 1 || t.stride(2) == 1, "paris_moe.", op, ": ", name,
+              "'s last dimension must be contiguous");
+}
+
+// A cache view [n_pages, Hkv, page_size, D]: any page stride, contiguous pages.
+struct CacheView {
+  int n_pages, Hkv, page_size, D, B, max_pages;
+  int64_t k_stride, v_stride, table_stride;
+};
+CacheView check_cache(const char* op, const Tensor& q, const Tensor& k, const Tensor& v,
+                      const Tensor& table, const Tensor& lens) {
+  for (const Tensor* t : {&k, &v}) {
+    const char* name = t == &k ? "k_pages" : "v_pages";
+    TORCH_CHECK(t->is_cuda() && t->device() == q.device(), "paris_moe.", op, ": ", name,
+                " must be a CUDA tensor on ", q.device());
+    TORCH_CHECK(t->scalar_type() == at::kBFloat16, "paris_moe.", op, ": ", name,
+                " must be bf16, got ", t->scalar_type());
+    TORCH_CHECK(t->dim() == 4, "paris_moe.", op, ": ", name,
+                " must be [n_pages, kv_heads, page_size, D]");
+    const int64_t d = t->size(3), ps = t->size(2);
+    TORCH_CHECK(t->numel() == 0 || ((d <= 1 || t->stride(3) == 1) && (ps <= 1 || t->stride(2) == d) &&
+                                    (t->size(1) <= 1 || t->stride(1) == ps * d)),
+                "paris_moe.", op, ": ", name, "'s last three dimensions must be contiguous");
+  }
+  TORCH_CHECK(k.sizes() == v.sizes(), "paris_moe.", op, ": k_pages and v_pages differ in shape");
+  check_int(op, "page_table", table, at::kInt, 2, q);
+  check_int(op, "kv_lens", lens, at::kInt, 1, q);
+  TORCH_CHECK(table.size(0) == lens.size(0), "paris_moe.", op, ": page_table has ", table.size(0),
+              " rows, kv_lens ", lens.size(0));
+  const int64_t page = k.size(1) * k.size(2) * k.size(3);
+  return {to_int(op, "n_pages", k.size(0)), to_int(op, "kv_heads", k.size(1)),
+          to_int(op, "page_size", k.size(2)), to_int(op, "D", k.size(3)),
+          to_int(op, "batch", lens.size(0)), to_int(op, "max_pages", table.size(1)),
+          k.size(0) <= 1 ? page : k.stride(0), v.size(0) <= 1 ? page : v.stride(0),
+          table.size(0) <= 1 ? table.size(1) : table.stride(0)};
+}
+
+const int32_t* i32(const Tensor& t) { return static_cast<const int32_t*>(t.data_ptr()); }
+int32_t* i32_mut(const Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); }
+uint16_t* pages_mut(const Tensor& t) { return static_cast<uint16_t*>(t.data_ptr()); }
+
+const int32_t* check_cu(const char* op, const Tensor& cu, const CacheView& c, const Tensor& q) {
+  check_int(op, "cu_q", cu, at::kInt, 1, q);
+  TORCH_CHECK(cu.size(0) == c.B + 1, "paris_moe.", op, ": cu_q has ", cu.size(0),
+              " entries, expected ", c.B + 1);
+  return i32(cu);
+}
+
+Tensor rope_append_cuda(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& positions,
+                        const Tensor& inv_freq, at::IntArrayRef sections, bool interleaved,
+                        const Tensor& k_pages, const Tensor& v_pages, const Tensor& page_table,
+                        const Tensor& kv_lens, const OptTensor& cu_q, const OptTensor& w_qnorm,
+                        const OptTensor& w_knorm, double eps, double mscale) {
+  const char* op = "rope_append";
+  check_rows(op, "q", q, q);
+  check_rows(op, "k", k, q);
+  check_rows(op, "v", v, q);
+  const CacheView c = check_cache(op, q, k_pages, v_pages, page_table, kv_lens);
+  const int T = to_int(op, "tokens", q.size(0)), Hq = to_int(op, "heads", q.size(1));
+  TORCH_CHECK(q.size(2) == c.D, "paris_moe.rope_append: q has D ", q.size(2), ", the cache ", c.D);
+  TORCH_CHECK(k.size(0) == T && k.size(1) == c.Hkv && k.size(2) == c.D && v.sizes() == k.sizes(),
+              "paris_moe.rope_append: k and v must be [", T, ", ", c.Hkv, ", ", c.D, "]");
+  check_int(op, "positions", positions, at::kLong, 2, q);
+  check_int(op, "inv_freq", inv_freq, at::kFloat, 1, q);
+  TORCH_CHECK(positions.size(1) == T, "paris_moe.rope_append: positions must be [axes, ", T, "]");
+  TORCH_CHECK(positions.size(0) >= 1 && positions.size(0) <= 4 &&
+                  int64_t(sections.size()) == positions.size(0),
+              "paris_moe.rope_append: one section for each of positions' 1 to 4 axes");
+  int sec[4] = {0, 0, 0, 0};
+  int64_t half = 0;
+  for (size_t i = 0; i < sections.size(); ++i) {
+    sec[i] = to_int(op, "section", sections[i]);
+    TORCH_CHECK(sec[i] >= 0, "paris_moe.rope_append: sections must not be negative");
+    half += sec[i];
+  }
+  TORCH_CHECK(half == inv_freq.size(0) && 2 * half <= c.D, "paris_moe.rope_append: sections add up to ",
+              half, ", inv_freq has ", inv_freq.size(0), " entries, D/2 is ", c.D / 2);
+  for (const OptTensor* w : {&w_qnorm, &w_knorm})
+    if (w->has_value()) {
+      check_bf16(op, "norm weight", **w, q, 1);
+      TORCH_CHECK((*w)->size(0) == c.D, "paris_moe.rope_append: norm weights must be [", c.D, "]");
+    }
+  TORCH_CHECK(cu_q.has_value() || T == c.B, "paris_moe.rope_append: ", T, " tokens for ", c.B,
+              " sequences need cu_q");
+  const int32_t* cu = cu_q.has_value() ? check_cu(op, *cu_q, c, q) : nullptr;
+  const c10::cuda::CUDAGuard guard(q.device());
+  Tensor out = at::empty({T, Hq, c.D}, q.options());
+  PMOE_CALL(pmoe_rope_append, bf(q), stride_of(q, 0), stride_of(q, 1), bf(k), stride_of(k, 0),
+            stride_of(k, 1), bf(v), stride_of(v, 0), stride_of(v, 1), T, Hq, c.Hkv, c.D,
+            static_cast<const int64_t*>(positions.data_ptr()),
+            positions.size(0) <= 1 ? int64_t(T) : positions.stride(0), int(positions.size(0)), sec,
+            interleaved ? 1 : 0, static_cast<const float*>(inv_freq.data_ptr()), int(2 * half),
+            w_qnorm.has_value() ? bf(*w_qnorm) : nullptr,
+            w_knorm.has_value() ? bf(*w_knorm) : nullptr, float(eps), float(mscale),
+            pages_mut(k_pages), pages_mut(v_pages), c.k_stride, c.v_stride, c.n_pages, c.page_size,
+            i32(page_table), c.table_stride, c.max_pages, i32(kv_lens), cu, c.B, bf_mut(out),
+            stream_of(q));
+  return out;
+}
+Tensor rope_append_meta(const Tensor& q, const Tensor&, const Tensor&, const Tensor&,
+                        const Tensor&, at::IntArrayRef, bool, const Tensor&, const Tensor&,
+                        const Tensor&, const Tensor&, const OptTensor&, const OptTensor&,
+                        const OptTensor&, double, double) {
+  return at::empty(q.sizes(), q.options());
+}
+
+Tensor attn_decode_cuda(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages,
+                        const Tensor& page_table, const Tensor& kv_lens, double scale,
+                        int64_t window, int64_t sinks) {
+  const char* op = "attn_decode";
+  check_rows(op, "q", q, q);
+  const CacheView c = check_cache(op, q, k_pages, v_pages, page_table, kv_lens);
+  const int Hq = to_int(op, "heads", q.size(1));
+  TORCH_CHECK(q.size(0) == c.B && q.size(2) == c.D, "paris_moe.attn_decode: q must be [", c.B,
+              ", heads, ", c.D, "]");
+  const c10::cuda::CUDAGuard guard(q.device());
+  Tensor out = at::empty({c.B, Hq, c.D}, q.options());
+  size_t nbytes = 0;
+  PMOE_CALL(pmoe_attn_decode_workspace, c.B, Hq, c.Hkv, c.D, &nbytes);
+  Tensor ws = at::empty({int64_t(nbytes)}, q.options().dtype(at::kByte));
+  PMOE_CALL(pmoe_attn_decode, bf(q), stride_of(q, 0), stride_of(q, 1), c.B, Hq, c.Hkv, c.D,
+            bf(k_pages), bf(v_pages), c.k_stride, c.v_stride, c.n_pages, c.page_size,
+            i32(page_table), c.table_stride, c.max_pages, i32(kv_lens), float(scale),
+            to_int(op, "window", window), to_int(op, "sinks", sinks), bf_mut(out), ws.data_ptr(),
+            nbytes, stream_of(q));
+  return out;
+}
+Tensor attn_decode_meta(const Tensor& q, const Tensor&, const Tensor&, const Tensor&,
+                        const Tensor&, double, int64_t, int64_t) {
+  return at::empty(q.sizes(), q.options());
+}
+
+Tensor attn_prefill_cuda(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages,
+                         const Tensor& page_table, const Tensor& kv_lens, const Tensor& cu_q,
+                         double scale, int64_t window, int64_t sinks) {
+  const char* op = "attn_prefill";
+  check_rows(op, "q", q, q);
+  const CacheView c = check_cache(op, q, k_pages, v_pages, page_table, kv_lens);
+  const int T = to_int(op, "tokens", q.size(0)), Hq = to_int(op, "heads", q.size(1));
+  TORCH_CHECK(q.size(2) == c.D, "paris_moe.attn_prefill: q has D ", q.size(2), ", the cache ", c.D);
+  const int32_t* cu = check_cu(op, cu_q, c, q);
+  const c10::cuda::CUDAGuard guard(q.device());
+  Tensor out = at::empty({T, Hq, c.D}, q.options());
+  PMOE_CALL(pmoe_attn_prefill, bf(q), stride_of(q, 0), stride_of(q, 1), T, Hq, c.Hkv, c.D,
+            bf(k_pages), bf(v_pages), c.k_stride, c.v_stride, c.n_pages, c.page_size,
+            i32(page_table), c.table_stride, c.max_pages, i32(kv_lens), cu, c.B, float(scale),
+            to_int(op, "window", window), to_int(op, "sinks", sinks), bf_mut(out), stream_of(q));
+  return out;
+}
+Tensor attn_prefill_meta(const Tensor& q, const Tensor&, const Tensor&, const Tensor&,
+                         const Tensor&, const Tensor&, double, int64_t, int64_t) {
+  return at::empty(q.sizes(), q.options());
+}
+
+// The bookkeeping tensors of a page pool.
+struct PoolView {
+  int n_pages, max_pages, S;
+  int64_t table_stride;
+};
+PoolView check_pool(const char* op, const Tensor& refs, const Tensor& tables) {
+  check_int(op, "refs", refs, at::kInt, 1, refs);
+  check_int(op, "tables", tables, at::kInt, 2, refs);
+  return {to_int(op, "n_pages", refs.size(0)), to_int(op, "max_pages", tables.size(1)),
+          to_int(op, "sequences", tables.size(0)),
+          tables.size(0) <= 1 ? tables.size(1) : tables.stride(0)};
+}
+void check_lens(const char* op, const Tensor& lens, const PoolView& p, const Tensor& refs) {
+  check_int(op, "lens", lens, at::kInt, 1, refs);
+  TORCH_CHECK(lens.size(0) == p.S, "paris_moe.", op, ": lens has ", lens.size(0),
+              " entries, tables ", p.S, " rows");
+}
+int check_list(const char* op, const char* name, const Tensor& t, int64_t n, const Tensor& refs) {
+  check_int(op, name, t, at::kInt, 1, refs);
+  TORCH_CHECK(t.size(0) == n, "paris_moe.", op, ": ", name, " has ", t.size(0),
+              " entries, expected ", n);
+  return to_int(op, name, n);
+}
+// The pool [n_pages, ..., page_size, D], contiguous.
+struct PageShape {
+  int chunks, page_size, D;
+};
+PageShape check_pages(const char* op, const Tensor& pages, const Tensor& refs) {
+  TORCH_CHECK(pages.is_cuda() && pages.device() == refs.device(), "paris_moe.", op,
+              ": pages must be a CUDA tensor on ", refs.device());
+  TORCH_CHECK(pages.scalar_type() == at::kBFloat16, "paris_moe.", op, ": pages must be bf16, got ",
+              pages.scalar_type());
+  TORCH_CHECK(pages.dim() >= 3 && pages.is_contiguous(), "paris_moe.", op,
+              ": pages must be contiguous [n_pages, ..., page_size, D]");
+  TORCH_CHECK(pages.size(0) == refs.size(0), "paris_moe.", op, ": pages holds ", pages.size(0),
+              " pages, refs ", refs.size(0));
+  int64_t chunks = 1;
+  for (int64_t i = 1; i + 2 < pages.dim(); ++i) chunks *= pages.size(i);
+  return {to_int(op, "chunks", chunks), to_int(op, "page_size", pages.size(pages.dim() - 2)),
+          to_int(op, "D", pages.size(pages.dim() - 1))};
+}
+Tensor pages_workspace(const Tensor& refs, int S, int n, int n_pages, size_t* nbytes) {
+  PMOE_CALL(pmoe_pages_workspace, S, n, n_pages, nbytes);
+  return at::empty({int64_t(*nbytes)}, refs.options().dtype(at::kByte));
+}
+
+Tensor pages_grow_cuda(const Tensor& refs, const Tensor& tables, const Tensor& lens,
+                       const Tensor& slots, const Tensor& add, int64_t page_size) {
+  const char* op = "pages_grow";
+  const PoolView p = check_pool(op, refs, tables);
+  check_lens(op, lens, p, refs);
+  const int n = check_list(op, "slots", slots, slots.numel(), refs);
+  check_list(op, "add", add, n, refs);
+  const c10::cuda::CUDAGuard guard(refs.device());
+  Tensor ok = at::empty({n}, refs.options());
+  size_t nbytes = 0;
+  Tensor ws = pages_workspace(refs, p.S, n, p.n_pages, &nbytes);
+  PMOE_CALL(pmoe_pages_grow, i32_mut(refs), p.n_pages, to_int(op, "page_size", page_size),
+            i32_mut(tables), p.table_stride, p.max_pages, p.S, i32_mut(lens), i32(slots), i32(add),
+            n, i32_mut(ok), ws.data_ptr(), nbytes, stream_of(refs));
+  return ok;
+}
+Tensor pages_grow_meta(const Tensor&, const Tensor&, const Tensor&, const Tensor& slots,
+                       const Tensor&, int64_t) {
+  return at::empty(slots.sizes(), slots.options().dtype(at::kInt));
+}
+
+Tensor pages_fork_cuda(const Tensor& pages, const Tensor& refs, const Tensor& tables,
+                       const Tensor& lens, const Tensor& src, const Tensor& dst,
+                       const Tensor& keep) {
+  const char* op = "pages_fork";
+  const PoolView p = check_pool(op, refs, tables);
+  check_lens(op, lens, p, refs);
+  const PageShape g = check_pages(op, pages, refs);
+  const int n = check_list(op, "src", src, src.numel(), refs);
+  check_list(op, "dst", dst, n, refs);
+  check_list(op, "keep", keep, n, refs);
+  const c10::cuda::CUDAGuard guard(refs.device());
+  Tensor ok = at::empty({n}, refs.options());
+  size_t nbytes = 0;
+  Tensor ws = pages_workspace(refs, p.S, n, p.n_pages, &nbytes);
+  PMOE_CALL(pmoe_pages_fork, pages_mut(pages), p.n_pages, g.chunks, g.page_size, g.D,
+            i32_mut(refs), i32_mut(tables), p.table_stride, p.max_pages, p.S, i32_mut(lens),
+            i32(src), i32(dst), i32(keep), n, i32_mut(ok), ws.data_ptr(), nbytes, stream_of(refs));
+  return ok;
+}
+Tensor pages_fork_meta(const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                       const Tensor& src, const Tensor&, const Tensor&) {
+  return at::empty(src.sizes(), src.options().dtype(at::kInt));
+}
+
+void pages_free_cuda(const Tensor& refs, const Tensor& tables, const Tensor& lens,
+                     const Tensor& slots, int64_t page_size, int64_t window, int64_t sinks) {
+  const char* op = "pages_free";
+  const PoolView p = check_pool(op, refs, tables);
+  check_lens(op, lens, p, refs);
+  const int n = check_list(op, "slots", slots, slots.numel(), refs);
+  const c10::cuda::CUDAGuard guard(refs.device());
+  PMOE_CALL(pmoe_pages_free, i32_mut(refs), p.n_pages, to_int(op, "page_size", page_size),
+            i32_mut(tables), p.table_stride, p.max_pages, p.S, i32_mut(lens), i32(slots), n,
+            to_int(op, "window", window), to_int(op, "sinks", sinks), stream_of(refs));
+}
+void pages_free_meta(const Tensor&, const Tensor&, const Tensor&, const Tensor&, int64_t, int64_t,
+                     int64_t) {}
+
+std::tuple<Tensor, Tensor> pages_compact_cuda(const Tensor& pages, const Tensor& refs,
+                                              const Tensor& tables) {
+  const char* op = "pages_compact";
+  const PoolView p = check_pool(op, refs, tables);
+  const PageShape g = check_pages(op, pages, refs);
+  const c10::cuda::CUDAGuard guard(refs.device());
+  Tensor live = at::empty({1}, refs.options()), remap = at::empty({p.n_pages}, refs.options());
+  size_t nbytes = 0;
+  Tensor ws = pages_workspace(refs, p.S, 0, p.n_pages, &nbytes);
+  PMOE_CALL(pmoe_pages_compact, pages_mut(pages), p.n_pages, g.chunks, g.page_size, g.D,
+            i32_mut(refs), i32_mut(tables), p.table_stride, p.max_pages, p.S, i32_mut(live),
+            i32_mut(remap), ws.data_ptr(), nbytes, stream_of(refs));
+  return {live, remap};
+}
+std::tuple<Tensor, Tensor> pages_compact_meta(const Tensor&, const Tensor& refs, const Tensor&) {
+  return {at::empty({1}, refs.options()), at::empty(refs.sizes(), refs.options())};
+}
+
 // CPU tensors: a clear error instead of a computation (there is no CPU path).
 [[noreturn]] void no_cpu(const char* op) {
   TORCH_CHECK(false, "paris_moe.", op, ": tensors must be CUDA (no CPU fallback)");
@@ -247,6 +558,35 @@ Tensor rmsnorm_cpu(const Tensor&, const Tensor&, double) { no_cpu("rmsnorm"); }
 RouteOut moe_route_cpu(const Tensor&, const Tensor&, const Tensor&, int64_t) {
   no_cpu("moe_route");
 }
+Tensor rope_append_cpu(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                       at::IntArrayRef, bool, const Tensor&, const Tensor&, const Tensor&,
+                       const Tensor&, const OptTensor&, const OptTensor&, const OptTensor&, double,
+                       double) {
+  no_cpu("rope_append");
+}
+Tensor attn_decode_cpu(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                       double, int64_t, int64_t) {
+  no_cpu("attn_decode");
+}
+Tensor attn_prefill_cpu(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                        const Tensor&, double, int64_t, int64_t) {
+  no_cpu("attn_prefill");
+}
+Tensor pages_grow_cpu(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                      int64_t) {
+  no_cpu("pages_grow");
+}
+Tensor pages_fork_cpu(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                      const Tensor&, const Tensor&) {
+  no_cpu("pages_fork");
+}
+void pages_free_cpu(const Tensor&, const Tensor&, const Tensor&, const Tensor&, int64_t, int64_t,
+                    int64_t) {
+  no_cpu("pages_free");
+}
+std::tuple<Tensor, Tensor> pages_compact_cpu(const Tensor&, const Tensor&, const Tensor&) {
+  no_cpu("pages_compact");
+}
 
 }  // namespace
 
@@ -264,6 +604,28 @@ TORCH_LIBRARY(paris_moe, m) {
   m.def(
       "moe_route(Tensor x, Tensor w_router, Tensor w_sh_gvec, int k) -> "
       "(Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def(
+      "rope_append(Tensor q, Tensor k, Tensor v, Tensor positions, Tensor inv_freq, "
+      "int[] sections, bool interleaved, Tensor(a!) k_pages, Tensor(b!) v_pages, "
+      "Tensor page_table, Tensor kv_lens, *, Tensor? cu_q=None, Tensor? w_qnorm=None, "
+      "Tensor? w_knorm=None, float eps=1e-6, float mscale=1.0) -> Tensor");
+  m.def(
+      "attn_decode(Tensor q, Tensor k_pages, Tensor v_pages, Tensor page_table, Tensor kv_lens, "
+      "float scale, int window=0, int sinks=0) -> Tensor");
+  m.def(
+      "attn_prefill(Tensor q, Tensor k_pages, Tensor v_pages, Tensor page_table, Tensor kv_lens, "
+      "Tensor cu_q, float scale, int window=0, int sinks=0) -> Tensor");
+  m.def(
+      "pages_grow(Tensor(a!) refs, Tensor(b!) tables, Tensor(c!) lens, Tensor slots, Tensor add, "
+      "int page_size) -> Tensor");
+  m.def(
+      "pages_fork(Tensor(a!) pages, Tensor(b!) refs, Tensor(c!) tables, Tensor(d!) lens, "
+      "Tensor src, Tensor dst, Tensor keep) -> Tensor");
+  m.def(
+      "pages_free(Tensor(a!) refs, Tensor(b!) tables, Tensor(c!) lens, Tensor slots, "
+      "int page_size, int window=0, int sinks=0) -> ()");
+  m.def(
+      "pages_compact(Tensor(a!) pages, Tensor(b!) refs, Tensor(c!) tables) -> (Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(paris_moe, CUDA, m) {
@@ -271,6 +633,13 @@ TORCH_LIBRARY_IMPL(paris_moe, CUDA, m) {
   m.impl("moe_layer", &moe_layer_cuda);
   m.impl("rmsnorm", &rmsnorm_cuda);
   m.impl("moe_route", &moe_route_cuda);
+  m.impl("rope_append", &rope_append_cuda);
+  m.impl("attn_decode", &attn_decode_cuda);
+  m.impl("attn_prefill", &attn_prefill_cuda);
+  m.impl("pages_grow", &pages_grow_cuda);
+  m.impl("pages_fork", &pages_fork_cuda);
+  m.impl("pages_free", &pages_free_cuda);
+  m.impl("pages_compact", &pages_compact_cuda);
 }
 
 TORCH_LIBRARY_IMPL(paris_moe, CPU, m) {
@@ -278,6 +647,13 @@ TORCH_LIBRARY_IMPL(paris_moe, CPU, m) {
   m.impl("moe_layer", &moe_layer_cpu);
   m.impl("rmsnorm", &rmsnorm_cpu);
   m.impl("moe_route", &moe_route_cpu);
+  m.impl("rope_append", &rope_append_cpu);
+  m.impl("attn_decode", &attn_decode_cpu);
+  m.impl("attn_prefill", &attn_prefill_cpu);
+  m.impl("pages_grow", &pages_grow_cpu);
+  m.impl("pages_fork", &pages_fork_cpu);
+  m.impl("pages_free", &pages_free_cpu);
+  m.impl("pages_compact", &pages_compact_cpu);
 }
 
 TORCH_LIBRARY_IMPL(paris_moe, Meta, m) {
@@ -285,4 +661,11 @@ TORCH_LIBRARY_IMPL(paris_moe, Meta, m) {
   m.impl("moe_layer", &moe_layer_meta);
   m.impl("rmsnorm", &rmsnorm_meta);
   m.impl("moe_route", &moe_route_meta);
+  m.impl("rope_append", &rope_append_meta);
+  m.impl("attn_decode", &attn_decode_meta);
+  m.impl("attn_prefill", &attn_prefill_meta);
+  m.impl("pages_grow", &pages_grow_meta);
+  m.impl("pages_fork", &pages_fork_meta);
+  m.impl("pages_free", &pages_free_meta);
+  m.impl("pages_compact", &pages_compact_meta);
 }

@@ -8,6 +8,15 @@
                                             sorted_slot, shared_gate)
     moe_layer(x, w_norm, eps, <7 weights>, top_k=8, flags=3) -> y
     rmsnorm(x, w_norm, eps) -> y
+    rope_append(q, k, v, positions, inv_freq, sections, interleaved, k_pages, v_pages,
+                page_table, kv_lens, *, cu_q=None, w_qnorm=None, w_knorm=None, eps=1e-6,
+                mscale=1.0) -> q       (k and v are written to the cache)
+    attn_decode(q, k_pages, v_pages, page_table, kv_lens, scale, window=0, sinks=0) -> out
+    attn_prefill(q, k_pages, v_pages, page_table, kv_lens, cu_q, scale, window=0, sinks=0) -> out
+    pages_grow(refs, tables, lens, slots, add, page_size) -> ok
+    pages_fork(pages, refs, tables, lens, src, dst, keep) -> ok
+    pages_free(refs, tables, lens, slots, page_size, window=0, sinks=0)
+    pages_compact(pages, refs, tables) -> (live, remap)
 
 The ops run on the current CUDA stream, allocate their outputs and workspace
 through PyTorch's caching allocator, never synchronise the host, and have
@@ -38,3 +47,10 @@ moe_block = torch.ops.paris_moe.moe_block
 moe_route = torch.ops.paris_moe.moe_route
 moe_layer = torch.ops.paris_moe.moe_layer
 rmsnorm = torch.ops.paris_moe.rmsnorm
+rope_append = torch.ops.paris_moe.rope_append
+attn_decode = torch.ops.paris_moe.attn_decode
+attn_prefill = torch.ops.paris_moe.attn_prefill
+pages_grow = torch.ops.paris_moe.pages_grow
+pages_fork = torch.ops.paris_moe.pages_fork
+pages_free = torch.ops.paris_moe.pages_free
+pages_compact = torch.ops.paris_moe.pages_compact

@@ -19,6 +19,7 @@ int ensure_device() {
   if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess)
     return PMOE_ERR_CUDA;
   if (major != 10) return PMOE_ERR_DEVICE;
+  if (attn_decode_init() != cudaSuccess) return PMOE_ERR_CUDA;
   g_ready[dev].store(1, std::memory_order_release);
   return PMOE_OK;
 }
@@ -74,7 +75,7 @@ int attn_args(AttnArgs* a, const uint16_t* q, int T, int Hq, int64_t q_st, int64
   if (T < 0 || window < 0 || sinks < 0) return PMOE_ERR_ARG;
   int s = check_cache(Hq, Hkv, D, kps, vps, n_pages, page_size, table_stride, max_pages, B);
   if (s != PMOE_OK) return s;
-  if (int64_t(T) * (Hq / Hkv) > 0x3fffffffLL) return PMOE_ERR_UNSUPPORTED;
+  if (int64_t(T) * Hq > 0x3fffffffLL) return PMOE_ERR_UNSUPPORTED;
   if (!stride_ok(q_st) || !stride_ok(q_sh)) return PMOE_ERR_ALIGN;
   if (T == 0) return PMOE_OK;
   if (!q || !out || !kv_lens || (n_pages > 0 && (!k || !v)) || (max_pages > 0 && !table))
@@ -202,15 +203,17 @@ int pmoe_attn_decode(const uint16_t* q, int64_t q_stride_t, int64_t q_stride_h, 
   if ((s = pmoe_attn_decode_workspace(B, Hq, Hkv, D, &need)) != PMOE_OK) return s;
   if (need > 0 && (!workspace || workspace_bytes < need)) return PMOE_ERR_WORKSPACE;
   if (!aligned16(workspace)) return PMOE_ERR_ALIGN;
+  // the line of work units is counted in 32 bits per sequence
+  if (int64_t(max_pages) * page_size / 16 * Hq > 0x7fffffffLL) return PMOE_ERR_UNSUPPORTED;
   if ((s = ensure_device()) != PMOE_OK) return s;
-  return launch_attn_rows(a, static_cast<cudaStream_t>(stream)) == cudaSuccess ? PMOE_OK
-                                                                               : PMOE_ERR_CUDA;
+  return launch_attn_decode(a, workspace, static_cast<cudaStream_t>(stream)) == cudaSuccess
+             ? PMOE_OK : PMOE_ERR_CUDA;
 }
 
 int pmoe_attn_decode_workspace(int B, int Hq, int Hkv, int D, size_t* bytes) {
   if (!bytes || B < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0) return PMOE_ERR_ARG;
   if (!head_dim_ok(D)) return PMOE_ERR_UNSUPPORTED;
-  *bytes = 0;
+  *bytes = attn_decode_ws_bytes(B, Hq, Hkv, D);
   return PMOE_OK;
 }
 

@@ -97,8 +97,14 @@ struct Pool {
   int32_t* lens;           // [S]
 };
 
+// CTAs of the decode kernel: one per SM of a B200.
+constexpr int kDecodeCtas = 148;
+
 cudaError_t launch_rope_append(const RopeArgs& a, cudaStream_t st);
 cudaError_t launch_attn_rows(const AttnArgs& a, cudaStream_t st);
+cudaError_t attn_decode_init();
+cudaError_t launch_attn_decode(const AttnArgs& a, void* ws, cudaStream_t st);
+size_t attn_decode_ws_bytes(int B, int Hq, int Hkv, int D);
 cudaError_t launch_pages_grow(const Pool& p, const int32_t* slots, const int32_t* add, int n,
                               int32_t* ok, int32_t* ws, cudaStream_t st);
 cudaError_t launch_pages_fork(const Pool& p, const int32_t* src, const int32_t* dst,

@@ -19,7 +19,7 @@ int ensure_device() {
   if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess)
     return PMOE_ERR_CUDA;
   if (major != 10) return PMOE_ERR_DEVICE;
-  if (attn_decode_init() != cudaSuccess) return PMOE_ERR_CUDA;
+  if (attn_decode_init() != cudaSuccess || attn_prefill_init() != cudaSuccess) return PMOE_ERR_CUDA;
   g_ready[dev].store(1, std::memory_order_release);
   return PMOE_OK;
 }
@@ -231,8 +231,8 @@ int pmoe_attn_prefill(const uint16_t* q, int64_t q_stride_t, int64_t q_stride_h,
                     max_pages, kv_lens, B, cu_q, scale, window, sinks, out);
   if (s != PMOE_OK || T == 0) return s;
   if ((s = ensure_device()) != PMOE_OK) return s;
-  return launch_attn_rows(a, static_cast<cudaStream_t>(stream)) == cudaSuccess ? PMOE_OK
-                                                                               : PMOE_ERR_CUDA;
+  return launch_attn_prefill(a, static_cast<cudaStream_t>(stream)) == cudaSuccess ? PMOE_OK
+                                                                                  : PMOE_ERR_CUDA;
 }
 
 int pmoe_pages_workspace(int S, int n, int n_pages, size_t* bytes) {

@@ -399,7 +399,7 @@ size_t pmoe_noalloc_scratch_bytes(void);
  * kv_lens[b] - (cu_q[b+1] - t).  Rows behind cu_q[B] belong to no sequence.
  * A table entry outside [0, n_pages) names no page: nothing is read or written
  * through it, and a row that sees such a key gets NaN.  Strides are in elements
- * (multiples of 8; the innermost dimension is contiguous).  The reference runs
+ * (positive multiples of 8; the innermost dimension is contiguous).  The reference runs
  * this half through the HF module (Qwen3_5MoeAttention) and its slot-pool cache
  * (engine/runtime/kv_cache.py:220); it has no operator of its own for any of it.
  *
@@ -442,13 +442,17 @@ int pmoe_attn_decode(const uint16_t* q, int64_t q_stride_t, int64_t q_stride_h, 
 
 /* The same for a packed batch of prompts or prompt chunks (cu_q): causal, with
  * the cached keys before them, the same window and sinks.  out [T][Hq][D]; rows of no
- * sequence, and rows at an index below zero, get zeros.  Deterministic. */
+ * sequence, and rows at an index below zero, get zeros.  Deterministic.  workspace as
+ * for pmoe_attn_decode, of pmoe_attn_prefill_workspace bytes (0 where none is needed). */
+int pmoe_attn_prefill_workspace(int T, int B, int Hq, int Hkv, int D, int page_size,
+                                int max_pages, size_t* bytes);
 int pmoe_attn_prefill(const uint16_t* q, int64_t q_stride_t, int64_t q_stride_h, int T, int Hq,
                       int Hkv, int D, const uint16_t* k_pages, const uint16_t* v_pages,
                       int64_t k_page_stride, int64_t v_page_stride, int n_pages, int page_size,
                       const int32_t* page_table, int64_t table_stride, int max_pages,
                       const int32_t* kv_lens, const int32_t* cu_q, int B, float scale,
-                      int window, int sinks, uint16_t* out, void* stream);
+                      int window, int sinks, uint16_t* out, void* workspace,
+                      size_t workspace_bytes, void* stream);
 
 /* ---- pages of the cache --------------------------------------------------------
  * Device-side state of a pool of n_pages pages, `chunks` blocks of [page_size][D]

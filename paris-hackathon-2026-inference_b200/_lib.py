@@ -83,7 +83,8 @@ SIGNATURES = {
     "pmoe_attn_decode": (_I, [_P, _L, _L, _I, _I, _I, _I, _P, _P, _L, _L, _I, _I, _P, _L, _I,
                               _P, _F, _I, _I, _P, _P, _SZ, _P]),
     "pmoe_attn_prefill": (_I, [_P, _L, _L, _I, _I, _I, _I, _P, _P, _L, _L, _I, _I, _P, _L, _I,
-                               _P, _P, _I, _F, _I, _I, _P, _P]),
+                               _P, _P, _I, _F, _I, _I, _P, _P, _SZ, _P]),
+    "pmoe_attn_prefill_workspace": (_I, [_I, _I, _I, _I, _I, _I, _I, ctypes.POINTER(_SZ)]),
     "pmoe_pages_workspace": (_I, [_I, _I, _I, ctypes.POINTER(_SZ)]),
     "pmoe_pages_grow": (_I, [_P, _I, _I, _P, _L, _I, _I, _P, _P, _P, _I, _P, _P, _SZ, _P]),
     "pmoe_pages_fork": (_I, [_P, _I, _I, _I, _I, _P, _P, _L, _I, _I, _P, _P, _P, _P, _I, _P,

@@ -38,7 +38,8 @@ int page_shift_of(int page_size) {
 }
 
 bool head_dim_ok(int D) { return D == 64 || D == 128 || D == 256; }
-bool stride_ok(int64_t s) { return s >= 0 && s % 8 == 0; }
+// A stride of a dimension of n entries, in elements: 16-byte steps.
+bool stride_ok(int64_t s, int64_t n) { return n <= 1 || (s > 0 && s % 8 == 0); }
 
 __nv_bfloat16* bfm(uint16_t* p) { return reinterpret_cast<__nv_bfloat16*>(p); }
 const __nv_bfloat16* bf(const uint16_t* p) { return reinterpret_cast<const __nv_bfloat16*>(p); }
@@ -76,7 +77,7 @@ int attn_args(AttnArgs* a, const uint16_t* q, int T, int Hq, int64_t q_st, int64
   int s = check_cache(Hq, Hkv, D, kps, vps, n_pages, page_size, table_stride, max_pages, B);
   if (s != PMOE_OK) return s;
   if (int64_t(T) * Hq > 0x3fffffffLL) return PMOE_ERR_UNSUPPORTED;
-  if (!stride_ok(q_st) || !stride_ok(q_sh)) return PMOE_ERR_ALIGN;
+  if (!stride_ok(q_st, T) || !stride_ok(q_sh, Hq)) return PMOE_ERR_ALIGN;
   if (T == 0) return PMOE_OK;
   if (!q || !out || !kv_lens || (n_pages > 0 && (!k || !v)) || (max_pages > 0 && !table))
     return PMOE_ERR_ARG;
@@ -142,9 +143,9 @@ int pmoe_rope_append(const uint16_t* q, int64_t q_stride_t, int64_t q_stride_h,
   }
   if (sum != rot / 2) return PMOE_ERR_ARG;
   if (!cu_q && T != B) return PMOE_ERR_ARG;
-  const int64_t strides[6] = {q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t, v_stride_h};
-  for (int64_t x : strides)
-    if (!stride_ok(x)) return PMOE_ERR_ALIGN;
+  if (!stride_ok(q_stride_t, T) || !stride_ok(q_stride_h, Hq) || !stride_ok(k_stride_t, T) ||
+      !stride_ok(k_stride_h, Hkv) || !stride_ok(v_stride_t, T) || !stride_ok(v_stride_h, Hkv))
+    return PMOE_ERR_ALIGN;
   if (T == 0) return PMOE_OK;
   if (!q || !k || !v || !q_out || !kv_lens || (rot > 0 && (!positions || !inv_freq)) ||
       (n_pages > 0 && (!k_pages || !v_pages)) || (max_pages > 0 && !page_table) ||
@@ -217,12 +218,22 @@ int pmoe_attn_decode_workspace(int B, int Hq, int Hkv, int D, size_t* bytes) {
   return PMOE_OK;
 }
 
+int pmoe_attn_prefill_workspace(int T, int B, int Hq, int Hkv, int D, int page_size, int max_pages,
+                                size_t* bytes) {
+  if (!bytes || T < 0 || B < 0 || max_pages < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0)
+    return PMOE_ERR_ARG;
+  if (!head_dim_ok(D) || page_shift_of(page_size) < 0 || Hq / Hkv > 128) return PMOE_ERR_UNSUPPORTED;
+  *bytes = T == 0 || B == 0 ? 0 : attn_prefill_ws_bytes(T, B, Hq, Hkv, D, int64_t(max_pages) * page_size);
+  return PMOE_OK;
+}
+
 int pmoe_attn_prefill(const uint16_t* q, int64_t q_stride_t, int64_t q_stride_h, int T, int Hq,
                       int Hkv, int D, const uint16_t* k_pages, const uint16_t* v_pages,
                       int64_t k_page_stride, int64_t v_page_stride, int n_pages, int page_size,
                       const int32_t* page_table, int64_t table_stride, int max_pages,
                       const int32_t* kv_lens, const int32_t* cu_q, int B, float scale, int window,
-                      int sinks, uint16_t* out, void* stream) {
+                      int sinks, uint16_t* out, void* workspace, size_t workspace_bytes,
+                      void* stream) {
   if (B < 1 && T > 0) return PMOE_ERR_ARG;
   if (!cu_q && T > 0) return PMOE_ERR_ARG;
   AttnArgs a{};
@@ -230,8 +241,11 @@ int pmoe_attn_prefill(const uint16_t* q, int64_t q_stride_t, int64_t q_stride_h,
                     v_page_stride, n_pages, page_size, Hkv, D, page_table, table_stride,
                     max_pages, kv_lens, B, cu_q, scale, window, sinks, out);
   if (s != PMOE_OK || T == 0) return s;
+  const size_t need = attn_prefill_ws_bytes(T, B, Hq, Hkv, D, int64_t(max_pages) * page_size);
+  if (need > 0 && (!workspace || workspace_bytes < need)) return PMOE_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return PMOE_ERR_ALIGN;
   if ((s = ensure_device()) != PMOE_OK) return s;
-  return launch_attn_prefill(a, static_cast<cudaStream_t>(stream)) == cudaSuccess ? PMOE_OK
+  return launch_attn_prefill(a, workspace, static_cast<cudaStream_t>(stream)) == cudaSuccess ? PMOE_OK
                                                                                   : PMOE_ERR_CUDA;
 }
 

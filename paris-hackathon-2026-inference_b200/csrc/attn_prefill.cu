@@ -1,19 +1,28 @@
 // Attention of packed prompts and prompt chunks over the paged cache, on the tensor cores.
 //   o = sum_j softmax_j(scale q.k_j) v_j over the keys that each row sees.
 //
-// One CTA per (128 rows of one sequence, key/value head).  The rows are tokens x the G
-// query heads that share the head, so one pass over K and V serves all of them.  Keys come in
-// tiles of 128:
+// One CTA, or a pair of CTAs, per (128 rows of one sequence for each CTA, key/value head).  The
+// rows are tokens x the G query heads that share the head, so one pass over K and V serves
+// all of them.  Keys come in tiles of 128:
 //   S = Q K^T         128 x 128, operands in shared memory, S in TMEM
-//   P = 2^(S c - m)   a thread per row reads its S from TMEM and writes P (bf16) over it
+//   P = 2^(S c - m)   a thread per row takes its S from TMEM into registers, which frees S for
+//                     the next tile's product at once, and writes P (bf16) to TMEM
 //   O += P V          A = P from TMEM, B = V from shared memory (dims contiguous), O in TMEM
-// The running maximum m of a row moves only when a tile's maximum exceeds it by more than 8
-// (in powers of two): weights then stay below 2^8, exact to the same relative rounding, and O
-// is rescaled rarely.  With two S buffers the product of tile j + 1 runs while the
-// weights of tile j are computed.
+// Two groups of four softmax warps take the even and the odd tiles, each with a P buffer of its
+// own, so that one group's exponentials run beside the other's maxima and beside the products.  The running maximum m
+// of a row passes from group to group through shared memory.  It moves only when a tile's
+// maximum exceeds it by more than 8 (in powers of two): weights then stay below 2^8, exact to
+// the same relative rounding, and O is rescaled rarely.
 //
-// Warps 0-3: softmax and epilogue (row = thread); warp 4: TMA; warp 5: MMA.  K and V travel
-// in 16 KiB chunks through one ring: K as 128 keys x 64 dims, V as 16384 / 2D keys x D dims.
+// In a pair each CTA fetches half of every tile (64 of the keys of K, half the dims of V) and the
+// products read both halves (cta_group::2): a lone CTA asks for 128 KiB of K and V per 2048
+// tensor cycles at D = 256, more than its 160 KiB ring hides at L2 latency.
+//
+// Warps 0-7: softmax and epilogue; warps 8 and 9: TMA of K (and Q) and of V, each through a ring
+// of 16 KiB chunks; warps 10 and 11: the products S and P V (a pair's first CTA issues for
+// both, and both CTAs' copies report to its barriers).
+//
+// Few rows: the keys are split over several CTAs (gridDim.y), whose parts join_kernel joins.
 //
 // Values that a row does not see must not reach its sum even where they are not finite, but
 // 0 x inf is NaN: in tiles at an edge of some row's sight, V rows that nobody sees or that
@@ -26,19 +35,20 @@ namespace pmoe {
 
 namespace {
 
-constexpr int kRows = 128, kTile = 128, kChunk = 16384;
+constexpr int kRows = 128, kTile = 128, kThreads = 384, kChunk = 16384;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kGrow = 8.f;  // powers of two that a row's maximum may lag behind
 
-template <int D> struct Cfg {
-  static constexpr int kS = D == 256 ? 2 : 1;           // S buffers
-  static constexpr int kSlots = D == 256 ? 10 : D == 128 ? 4 : 5;
-  static constexpr int kCtas = D == 256 ? 1 : 2;        // CTAs per SM
-  static constexpr int kCols = D == 256 ? 512 : 256;    // TMEM columns
-  static constexpr int kKc = D / 64;                    // K chunks of a tile
-  static constexpr int kVr = kChunk / (2 * D);          // keys of a V chunk
-  static constexpr int kVc = kTile / kVr;               // V chunks of a tile
-  static constexpr int kSmem = 1024 + kRows * D * 2 + kSlots * kChunk;
+template <int D, bool PAIR> struct Cfg {
+  static constexpr int kN = PAIR ? 2 : 1;               // CTAs that share a tile
+  static constexpr int kS = D == 256 ? 1 : 2;           // S buffers: 512 columns of TMEM hold
+                                                        // O [D], S [kS][128], P [2][64]
+  static constexpr int kSlots = (229376 - kRows * D * 2) / (2 * kChunk);  // of each ring
+  // K chunk: [kKg groups of 64 dims][kKr keys][128 bytes]; V chunk: [kVg][kVr keys][128 bytes]
+  static constexpr int kKr = kTile / kN, kKg = kChunk / (kKr * 128), kKc = D / (64 * kKg);
+  static constexpr int kVg = D / (64 * kN), kVr = kChunk / (kVg * 128), kVc = kTile / kVr;
+  static constexpr int kSmem = 1024 + kRows * D * 2 + 2 * kSlots * kChunk;
+  static_assert(kKc * kChunk * kN == kTile * D * 2 && kVc == kKc, "");
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -46,24 +56,104 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int row, int cg,
-                                        int h, int page, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(row), "r"(cg), "r"(h), "r"(page),
-      "r"(smem_u32(bar))
-      : "memory");
+// Two 32-bit operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)),
+        "l"(reinterpret_cast<uint64_t&>(c)));
+  return d;
 }
-// D[tmem] (+)= A[tmem] * B[smem], A bf16 pairs in 32-bit columns.
-__device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc,
-                                        uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return d;
+}
+// Boxes of the cache and of Q; `bar` is a shared::cluster address (a pair's copies may complete
+// on the first CTA's barrier).
+template <bool PAIR>
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int row, int cg,
+                                        int h, int page, uint32_t bar) {
+  if (PAIR)
+    asm volatile(
+        "cp.async.bulk.tensor.5d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(row), "r"(cg), "r"(h), "r"(page), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(row), "r"(cg), "r"(h), "r"(page), "r"(bar)
+        : "memory");
+}
+template <bool PAIR>
+__device__ __forceinline__ void tma_load_q(uint32_t dst, const CUtensorMap* map, int d, int head,
+                                           int token, uint32_t bar) {
+  if (PAIR)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(d), "r"(head), "r"(token), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(d), "r"(head), "r"(token), "r"(bar)
+        : "memory");
+}
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
-      : "memory");
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
+}
+// Shared-memory descriptors in two words: the low one holds the address and the leading
+// offset and steps with plain 32-bit additions; the high one (stride 1024 bytes, version 1,
+// 128-byte swizzle) is the same for all operands here.
+constexpr uint32_t kDescHi = (1024u >> 4) | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t leading) {
+  return (saddr & 0x3FFFFu) >> 4 | (leading >> 4) << 16;
+}
+// D[tmem] (+)= A[smem] * B[smem]; with a TS prefix A is in TMEM, bf16 pairs in 32-bit columns.
+#define PMOE_UMMA(GROUP, ADECL, AOP, AVAL)                                              \
+  asm volatile(                                                                               \
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"                                             \
+      "setp.ne.b32 p, %4, 0;\n\t" ADECL                                                       \
+      "mov.b64 b, {%2, %5};\n\t"                                                              \
+      "tcgen05.mma.cta_group::" GROUP ".kind::f16 [%0], " AOP ", b, %3, p;\n\t}" ::"r"(d),    \
+      "r"(AVAL), "r"(b), "r"(idesc), "r"(accumulate), "n"(kDescHi)                            \
+      : "memory")
+template <bool PAIR>
+__device__ __forceinline__ void umma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc,
+                                        uint32_t accumulate) {
+  if (PAIR)
+    PMOE_UMMA("2", "mov.b64 a, {%1, %5};\n\t", "a", a);
+  else
+    PMOE_UMMA("1", "mov.b64 a, {%1, %5};\n\t", "a", a);
+}
+template <bool PAIR>
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc,
+                                        uint32_t accumulate) {
+  if (PAIR)
+    PMOE_UMMA("2", "", "[%1]", a);
+  else
+    PMOE_UMMA("1", "", "[%1]", a);
+}
+#undef PMOE_UMMA
+template <bool PAIR> __device__ __forceinline__ void commit(uint64_t* bar) {
+  if (PAIR)
+    umma_commit_pair_both(bar);
+  else
+    umma_commit(bar);
 }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
@@ -86,32 +176,39 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&p);
 }
-// V chunk [D/64][kVr keys][128 bytes], swizzled, as the B operand with dims contiguous: next
-// 64 dims `group` bytes on (leading), next 8 keys 1024 bytes on (stride).
-__device__ __forceinline__ uint64_t sdesc_mn_sw128(uint32_t saddr, uint32_t group) {
-  uint64_t d = 0;
-  d |= uint64_t((saddr & 0x3FFFFu) >> 4);
-  d |= uint64_t(group >> 4) << 16;
-  d |= uint64_t(1024 >> 4) << 32;
-  d |= uint64_t(1) << 46;
-  d |= uint64_t(2) << 61;
-  return d;
-}
-// bar.red over the softmax warps: whether any thread says yes.
-__device__ __forceinline__ bool softmax_any(bool x) {
+// Whether any of the barrier's n threads says yes.
+__device__ __forceinline__ bool bar_any(int id, int n, bool x) {
   uint32_t r;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.u32 p, %1, 0;\n\t"
-      "bar.red.or.pred q, 1, 128, p;\n\t"
+      "setp.ne.u32 p, %3, 0;\n\t"
+      "bar.red.or.pred q, %1, %2, p;\n\t"
       "selp.u32 %0, 1, 0, q;\n\t}"
       : "=r"(r)
-      : "r"(uint32_t(x))
+      : "r"(id), "r"(n), "r"(uint32_t(x))
       : "memory");
   return r != 0;
 }
+__device__ __forceinline__ void bar_arrive(int id, int n) {
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(n) : "memory");
+}
+// Arrive on a barrier of the MMA warps.  What it announces is in TMEM (wait::ld, wait::st and the
+// tcgen05 fence order it); nothing else has been written, so no release: at cluster scope it
+// would wait for all of the thread's stores (1276 cycles a tile, measured).
+template <bool PAIR> __device__ __forceinline__ void tmem_signal(uint64_t* bar) {
+  if (PAIR)
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(
+                     mapa_shared(smem_u32(bar), 0))
+                 : "memory");
+  else
+    mbar_arrive(bar);
+}
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity));
+}
+// Whether a 32-bit word holds a bf16 that is not finite.
+__device__ __forceinline__ bool nonfinite2(uint32_t x) {
+  return (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u;
 }
 
 // Block x's rows: slots of a sequence begin at cu[b] / tokens + b, which leaves each
@@ -120,359 +217,484 @@ struct TileOf {
   int b, t0, n, p0, len;  // sequence, first packed row, tokens, index of the first, keys
   bool over;
 };
+// (A whole warp calls this: it searches 32 places at a time.)
 __device__ __forceinline__ bool find_tile(const AttnArgs& a, int per, int x, TileOf* o) {
-  const int B = a.kv.B;
-  if (x < a.cu_q[0] / per) return false;
-  int lo = 0, hi = B;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (a.cu_q[mid] / per + mid <= x) lo = mid; else hi = mid;
-  }
-  const int c0 = a.cu_q[lo], c1 = min(a.cu_q[lo + 1], a.T);
+  const int lane = threadIdx.x & 31;
+  int lo = 0, n = a.kv.B;  // the last b in [lo, lo + n) whose slots begin at or before x
+  do {
+    const int step = (n + 31) / 32, b = lo + lane * step;
+    const bool before = lane * step < n && a.cu_q[b] / per + b <= x;
+    const int k = __popc(__ballot_sync(0xffffffffu, before));
+    if (k == 0) return false;
+    n = min(step, n - (k - 1) * step);
+    lo += (k - 1) * step;
+  } while (n > 1);
+  const int c0 = a.cu_q[lo], c1 = min(a.cu_q[lo + 1], a.T), len = a.kv.kv_lens[lo];
   const int i = x - (c0 / per + lo);
-  if (c0 < 0 || i < 0 || i > (c1 - c0 - 1) / per || c1 <= c0) return false;
+  if (c0 < 0 || c1 <= c0 || i < 0 || i > (c1 - c0 - 1) / per) return false;
   o->b = lo;
   o->t0 = c0 + i * per;
   o->n = min(per, c1 - o->t0);
-  o->len = kv_len_of(a.kv.kv_lens[lo], a.kv.max_pages, a.kv.page_shift, &o->over);
+  o->len = kv_len_of(len, a.kv.max_pages, a.kv.page_shift, &o->over);
   o->p0 = o->len - (c1 - o->t0);
   return true;
 }
 
-template <int D>
-__global__ void __launch_bounds__(192, Cfg<D>::kCtas) attn_prefill_kernel(
-    const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-    const AttnArgs a) {
-  using C = Cfg<D>;
+// Rows of no sequence get zeros (all blocks of the grid share them).
+__device__ __forceinline__ void zero_rows(const AttnArgs& a) {
+  const int lo = min(max(a.cu_q[0], 0), a.T), hi = min(max(a.cu_q[a.kv.B], lo), a.T);
+  if (lo == 0 && hi == a.T) return;
+  const int64_t row = int64_t(a.Hq) * a.kv.D / 8;  // 16-byte pieces of a packed row
+  const int64_t id = (int64_t(blockIdx.y) * gridDim.x + blockIdx.x) * kThreads + threadIdx.x;
+  const int64_t step = int64_t(gridDim.x) * gridDim.y * kThreads;
+  uint4* out = reinterpret_cast<uint4*>(a.out);
+  for (int64_t i = id; i < lo * row; i += step) out[i] = uint4{0, 0, 0, 0};
+  for (int64_t i = hi * row + id; i < a.T * row; i += step) out[i] = uint4{0, 0, 0, 0};
+}
+
+// Parts of a split call: O [128][D] of (block x, split y), not yet divided, then each row's
+// (m, l), m in powers of two.
+struct Parts {
+  float* o;
+  float2* ml;
+};
+__host__ __device__ inline Parts parts_of(void* ws, int64_t blocks, int D) {
+  float* o = static_cast<float*>(ws);
+  return {o, reinterpret_cast<float2*>(o + blocks * kRows * D)};
+}
+
+template <int D, bool PAIR>
+__global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(
+    const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+    const __grid_constant__ CUtensorMap map_v, const AttnArgs a, void* ws) {
+  using C = Cfg<D, PAIR>;
   extern __shared__ char smem_raw[];
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   char* s_q = smem;                    // [D/64][128 rows][128 bytes], swizzled
-  char* s_ring = smem + kRows * D * 2;
-  __shared__ uint64_t full[C::kSlots], empty[C::kSlots], s_full[C::kS], p_ready[C::kS], pv_done[2], q_ready;
+  char* s_k = smem + kRows * D * 2;    // the rings
+  char* s_v = s_k + C::kSlots * kChunk;
+  // full: a chunk has landed, in both CTAs (the first CTA's barrier counts); local: this CTA's
+  // part of a V chunk that its softmax warps clean first (other chunks pass it at once)
+  __shared__ uint64_t k_full[C::kSlots], k_empty[C::kSlots];
+  __shared__ uint64_t v_full[C::kSlots], v_empty[C::kSlots], v_local[C::kSlots];
+  __shared__ uint64_t s_full[2], s_free[C::kS], p_ready[2][2], pv_done[2], q_full;
   __shared__ uint32_t s_tmem;
   __shared__ int s_first;              // tile 0 adds to O (set to zero before) instead of setting it
-  __shared__ uint32_t s_bad[4];        // keys of the tile whose V row is not finite
+  __shared__ uint16_t s_bad[2][8];     // per group: keys of the tile whose V row is not finite
+  __shared__ float s_m[kRows], s_l[2][kRows];
 
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // (shuffled, so that the compiler sees one value per warp and keeps the roles' addresses
+  // in uniform registers)
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+  const int rank = PAIR ? int(cluster_ctarank()) : 0;
   const int G = a.Hq / a.kv.Hkv, per = kRows / G;
-  const int h = blockIdx.x % a.kv.Hkv;
-  const int x = int(gridDim.x / a.kv.Hkv) - 1 - int(blockIdx.x / a.kv.Hkv);  // late tiles, the longest, first
+  const int block = blockIdx.x / C::kN, blocks = gridDim.x / C::kN;
+  const int h = block % a.kv.Hkv;
+  const int x = blocks / a.kv.Hkv - 1 - block / a.kv.Hkv;  // late tiles, the longest, first
   TileOf tile;
-  if (!find_tile(a, per, x, &tile)) return;
+  if (!find_tile(a, per * C::kN, x, &tile)) {  // both CTAs of a pair, or none
+    zero_rows(a);
+    return;
+  }
 
-  // keys that some row sees: [0, sink_any) and [lo_any, last]
+  // keys that some row sees: [0, sink_any) and [lo_any, p_last]
   const int p_last = tile.p0 + tile.n - 1, p_first = max(tile.p0, 0);
   int lo_any = 0, sink_any = 0, lo_max = 0, sink_all = 0;
-  int n_tiles = 0, ns = 0, w0 = 0;
+  int n_tiles = 0, ns = 0, w0 = 0, j_lo = 0;
   if (p_last >= 0 && !tile.over) {
     visible_keys(p_first, a.window, a.sinks, &lo_any, &sink_all);
     visible_keys(p_last, a.window, a.sinks, &lo_max, &sink_any);
     ns = (sink_any + kTile - 1) / kTile;
     w0 = max(lo_any / kTile, ns);
     n_tiles = ns + p_last / kTile + 1 - w0;
+    if (gridDim.y > 1) {  // this CTA's share of the keys
+      j_lo = int(int64_t(n_tiles) * blockIdx.y / gridDim.y);
+      n_tiles = int(int64_t(n_tiles) * (blockIdx.y + 1) / gridDim.y) - j_lo;
+    }
   }
-  auto tile_key = [&](int j) { return (j < ns ? j : w0 + j - ns) * kTile; };
+  auto tile_key = [&](int j) {
+    j += j_lo;
+    return (j < ns ? j : w0 + j - ns) * kTile;
+  };
 
-  if (warp == 5) {
-    tmem_alloc(&s_tmem, C::kCols);
-    tmem_relinquish();
+  // a missing page where some row looks: every tile is an edge (found below)
+  auto edge_of = [&](int j, bool hole) {  // may some row not see some key of the tile?
+    const int k0 = tile_key(j);
+    return hole || tile.p0 < 0 || k0 + kTile - 1 > tile.p0 || (k0 < lo_max && k0 + kTile > sink_all);
+  };
+
+  if (warp == 10) {
+    if (PAIR) {
+      tmem_alloc_pair(&s_tmem, 512);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(&s_tmem, 512);
+      tmem_relinquish();
+    }
   }
   if (tid == 0) {
     for (int i = 0; i < C::kSlots; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 1);
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 1);
+      mbar_init(&v_local[i], 1);
     }
-    for (int i = 0; i < C::kS; ++i) {
+    for (int i = 0; i < C::kS; ++i) mbar_init(&s_free[i], 4 * C::kN);
+    for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_ready[i], 4);
+      mbar_init(&p_ready[i][0], 4 * C::kN);
+      mbar_init(&p_ready[i][1], 4 * C::kN);
+      mbar_init(&pv_done[i], 1);
     }
-    mbar_init(&pv_done[0], 1);
-    mbar_init(&pv_done[1], 1);
-    mbar_init(&q_ready, 4);
+    mbar_init(&q_full, 1);
     s_first = 0;
     mbar_fence_init();
   }
   tc_fence_before();
-  __syncthreads();
+  if (PAIR)
+    cluster_sync_all();
+  else
+    __syncthreads();
   tc_fence_after();
-  const uint32_t tm_o = s_tmem, tm_s = s_tmem + D;  // O [D columns], then the S buffers
+  const uint32_t tm_o = __shfl_sync(0xffffffffu, s_tmem, 0), tm_p = tm_o + D, tm_s = tm_p + 128;
 
-  if (warp == 4) {
-    // ---- TMA: K0, (K1, V0), (K2, V1) ... with two S buffers, K0, V0, K1, V1 ... with one
-    int seq = 0;
-    bool ok = true;
-    int page[2] = {-1, -1};  // lane i: page of the tile's i-th page, of the tiles j and j + 1
-    const int ps = 1 << a.kv.page_shift, per_tile = max(1, kTile / ps);
-    auto pages_of = [&](int j) {
-      const int k0 = tile_key(j);
-      return j < n_tiles && lane < per_tile ? page_of(a.kv, tile.b, k0 + lane * ps) : -1;
-    };
-    auto slot_open = [&]() {
-      const int s = seq % C::kSlots;
-      if (seq >= C::kSlots) ok = ok && warp_wait(&empty[s], (seq / C::kSlots - 1) & 1);
-      return s;
-    };
-    auto load_k = [&](int j, int mine) {
-      const int k0 = tile_key(j), rows = min(ps, kTile);
-      const int at = mine < 0 ? a.kv.n_pages : mine, row = ps > kTile ? k0 & (ps - 1) : 0;
-      for (int c = 0; c < C::kKc && ok; ++c, ++seq) {
-        const int s = slot_open();
-        if (!ok) break;
-        if (lane == 0) mbar_arrive_expect_tx(&full[s], kChunk);
+  // (384 threads start with 168 registers each; the softmax warps hold a row of S.)
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    if (warp < 10) {
+      // ---- TMA of one operand
+      const bool is_v = warp == 9;
+      uint64_t* full = is_v ? v_full : k_full;
+      uint64_t* empty = is_v ? v_empty : k_empty;
+      const uint32_t ring = smem_u32(is_v ? s_v : s_k);
+      const uint32_t first_full = mapa_shared(smem_u32(full), 0);  // the first CTA's barriers
+      const int sh = a.kv.page_shift, ps = 1 << sh, per_tile = kTile >> sh;
+      // this CTA's part of a tile: K: half the keys in a pair; V: half the dims
+      const int keys = is_v ? C::kVr : C::kKr, groups = is_v ? C::kVg : C::kKg;
+      const int rows = min(ps, keys), grp = lane % groups, r = lane / groups * rows;  // this lane's box
+      if (!is_v && n_tiles > 0) {
+        // Q: rows = tokens x heads, as they lie.  Rows behind the tile's tokens are other
+        // tokens' or zeros, and their results are not used.
+        if (lane == 0 && rank == 0) mbar_arrive_expect_tx(&q_full, C::kN * per * G * D * 2);
         __syncwarp();
-        if (lane < per_tile)
-          tma_box(smem_u32(s_ring + s * kChunk) + lane * rows * 128, &map_k, row, c, h, at, &full[s]);
+        if (lane < D / 64)
+          tma_load_q<PAIR>(smem_u32(s_q + lane * kRows * 128), &map_q, lane * 64, h * G,
+                           tile.t0 + rank * per, mapa_shared(smem_u32(&q_full), 0));
       }
-    };
-    auto load_v = [&](int j, int mine) {
-      const int rows = min(ps, C::kVr), boxes = C::kVr / rows;
-      for (int c = 0; c < C::kVc && ok; ++c, ++seq) {
-        const int s = slot_open();
-        if (!ok) break;
-        if (lane == 0) mbar_arrive_expect_tx(&full[s], kChunk);
-        __syncwarp();
-        // box i: rows of dims group i % (D/64)
-        const int i = lane, cg = i % (D / 64), r = i / (D / 64) * rows;
-        const int key = c * C::kVr + r;  // in the tile
-        const int pg = __shfl_sync(0xffffffffu, mine, min(key >> a.kv.page_shift, 31));
-        if (i < boxes * (D / 64))
-          tma_box(smem_u32(s_ring + s * kChunk) + cg * C::kVr * 128 + r * 128, &map_v,
-                  key & (ps - 1), cg, h, pg < 0 ? a.kv.n_pages : pg, &full[s]);
+      auto pages_of = [&](int j) {  // lane i: the tile's i-th page
+        return j < n_tiles && lane < per_tile ? page_of(a.kv, tile.b, tile_key(j) + lane * ps) : -1;
+      };
+      int next = pages_of(0), slot = 0, use = 0;
+      bool hole = false;
+      if (is_v && n_tiles > 0) {
+        for (int i = lane; i < (sink_any + ps - 1) >> sh; i += 32) hole |= page_of(a.kv, tile.b, i << sh) < 0;
+        for (int i = (lo_any >> sh) + lane; i <= p_last >> sh; i += 32)
+          hole |= page_of(a.kv, tile.b, i << sh) < 0;
+        hole = __any_sync(0xffffffffu, hole);
       }
-    };
-    page[0] = pages_of(0);
-    if (n_tiles > 0) load_k(0, page[0]);
-    for (int j = 0; j < n_tiles && ok; ++j) {
-      page[1] = pages_of(j + 1);
-      if (C::kS == 2 && j + 1 < n_tiles) load_k(j + 1, page[1]);
-      load_v(j, page[0]);
-      if (C::kS == 1 && j + 1 < n_tiles) load_k(j + 1, page[1]);
-      page[0] = page[1];
-    }
-    if (!ok)  // a wait ran out: let the copies land before the CTA ends
-      for (int q = max(0, seq - C::kSlots); q < seq; ++q)
-        mbar_wait(&full[q % C::kSlots], (q / C::kSlots) & 1);
-  } else if (warp == 5) {
-    // ---- MMA, one thread
-    if (lane == 0 && n_tiles > 0) {
-      constexpr uint32_t idesc_s = idesc_bf16_f32(kRows, kTile);
-      constexpr uint32_t idesc_o = idesc_bf16_f32(kRows, D) | 1u << 16;  // B with dims contiguous
+      bool ok = true;
       int seq = 0;
-      bool ok = mbar_wait(&q_ready, 0);
-      auto qk = [&](int j) {
-        for (int c = 0; c < C::kKc && ok; ++c, ++seq) {
-          const int s = seq % C::kSlots;
-          ok = mbar_wait(&full[s], (seq / C::kSlots) & 1);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t ka = smem_u32(s_ring + s * kChunk), qa = smem_u32(s_q) + c * kRows * 128;
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_bf16(tm_s + (j % C::kS) * kTile, sdesc_k_sw128(qa + k * 32),
-                      sdesc_k_sw128(ka + k * 32), idesc_s, c > 0 || k > 0);
-          umma_commit(&empty[s]);
-        }
-        if (ok) umma_commit(&s_full[j % C::kS]);
-      };
-      auto pv = [&](int j) {
-        ok = ok && mbar_wait(&p_ready[j % C::kS], (j / C::kS) & 1);
-        if (!ok) return;
-        tc_fence_after();
-        const bool add = j > 0 || *(volatile int*)&s_first;
-        for (int c = 0; c < C::kVc && ok; ++c, ++seq) {
-          const int s = seq % C::kSlots;
-          ok = mbar_wait(&full[s], (seq / C::kSlots) & 1);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t va = smem_u32(s_ring + s * kChunk);
-#pragma unroll
-          for (int k = 0; k < C::kVr / 16; ++k)
-            umma_ts(tm_o, tm_s + (j % C::kS) * kTile + (c * C::kVr + k * 16) / 2,
-                    sdesc_mn_sw128(va + k * 2048, C::kVr * 128), idesc_o, add || c > 0 || k > 0);
-          umma_commit(&empty[s]);
-        }
-        if (ok) umma_commit(&pv_done[j & 1]);
-      };
-      if (C::kS == 2 && ok) qk(0);
       for (int j = 0; j < n_tiles && ok; ++j) {
-        if (C::kS == 2) {
-          if (j + 1 < n_tiles) qk(j + 1);
-        } else {
-          qk(j);
+        const int page = next;
+        next = pages_of(j + 1);
+        const bool clean = is_v && edge_of(j, hole);
+        for (int c = 0; c < C::kKc; ++c, ++seq) {
+          if (use > 0) ok = warp_wait(&empty[slot], (use - 1) & 1);
+          if (!ok) break;
+          if (lane == 0) {
+            if (clean) {
+              if (rank == 0) mbar_arrive(&full[slot]);
+              mbar_arrive_expect_tx(&v_local[slot], kChunk);
+            } else {
+              if (rank == 0) mbar_arrive_expect_tx(&full[slot], C::kN * kChunk);
+              if (is_v) mbar_arrive(&v_local[slot]);
+            }
+          }
+          __syncwarp();
+          const int key = (is_v ? c * C::kVr : rank * C::kKr) + r;  // in the tile
+          const int cg = (is_v ? rank * C::kVg : c * C::kKg) + grp;
+          const int at = __shfl_sync(0xffffffffu, page, min(key >> sh, 31));
+          if (r < keys)
+            tma_box<PAIR>(ring + slot * kChunk + (grp * keys + r) * 128, is_v ? &map_v : &map_k,
+                          key & (ps - 1), cg, h, at < 0 ? a.kv.n_pages : at,  // no page: zeros
+                          clean ? smem_u32(&v_local[slot]) : first_full + slot * 8);
+          slot = slot + 1 == C::kSlots ? 0 : slot + 1;
+          use += slot == 0;
         }
-        if (ok) pv(j);
       }
+      if (!ok)  // a wait ran out: let the copies land before the CTA ends
+        for (int q = max(0, seq - C::kSlots); q < seq; ++q) {
+          if (rank == 0) mbar_wait(&full[q % C::kSlots], (q / C::kSlots) & 1);
+          if (is_v) mbar_wait(&v_local[q % C::kSlots], (q / C::kSlots) & 1);
+        }
+    } else {
+      // ---- the products: a warp each for S and P V walks and waits, one lane issues.  (A warp
+      // of its own for each: one warp for both spent 3300 cycles a tile on waits and issue, the
+      // tensor cores 2048.  The whole warp, so that the addresses are uniform: issued from one
+      // lane's branch, with descriptors built one by one, a product took 130 to 310 cycles to
+      // issue.)  The waits acquire at CTA scope also for what the pair's other CTA signals:
+      // these warps themselves read none of that data (the tensor cores do, after the other CTA's
+      // own waits and proxy fences), and a cluster-scope acquire costs some 400 cycles.
+      if (rank == 0 && n_tiles > 0) {
+        int slot = 0, phase = 0;
+        bool ok = true;
+        auto chunk_next = [&]() {
+          slot = slot + 1 == C::kSlots ? 0 : slot + 1;
+          phase ^= slot == 0;
+        };
+        if (warp == 10) {
+          // A negative scale turns the sign of Q (bit 13).
+          const uint32_t idesc = idesc_bf16_f32(kRows * C::kN, kTile) | (a.scale < 0.f ? 1u << 13 : 0u);
+          const uint32_t ring = smem_u32(s_k), q_lo = desc_lo(smem_u32(s_q), 0);
+          ok = warp_wait(&q_full, 0);
+          for (int j = 0; j < n_tiles && ok; ++j) {
+            const int buf = j % C::kS;
+            const uint32_t d = tm_s + buf * kTile;
+            if (j >= C::kS) ok = warp_wait(&s_free[buf], (j / C::kS - 1) & 1);
+#pragma unroll 1
+            for (int c = 0; c < C::kKc; ++c) {
+              ok = ok && warp_wait(&k_full[slot], phase);
+              tc_fence_after();
+              if (!ok) break;
+              const uint32_t qa = q_lo + c * C::kKg * kRows * 8, ka = desc_lo(ring + slot * kChunk, 0);
+              if (elect_one()) {
+#pragma unroll
+                for (int k = 0; k < 4 * C::kKg; ++k)
+                  umma_ss<PAIR>(d, qa + (k >> 2) * kRows * 8 + (k & 3) * 2,
+                                ka + (k >> 2) * C::kKr * 8 + (k & 3) * 2, idesc, k > 0 ? 1 : c > 0);
+                commit<PAIR>(&k_empty[slot]);
+                if (c == C::kKc - 1) commit<PAIR>(&s_full[j & 1]);
+              }
+              __syncwarp();
+              chunk_next();
+            }
+          }
+        } else {
+          constexpr uint32_t idesc = idesc_bf16_f32(kRows * C::kN, D) | 1u << 16;  // B: dims contiguous
+          const uint32_t ring = smem_u32(s_v);
+          for (int j = 0; j < n_tiles && ok; ++j) {
+            const uint32_t p = tm_p + (j & 1) * 64;
+            uint32_t add = 1;
+#pragma unroll 1
+            for (int c = 0; c < C::kVc; ++c) {
+              ok = ok && warp_wait(&v_full[slot], phase);
+              const uint32_t v_lo = desc_lo(ring + slot * kChunk, C::kVr * 128);
+              constexpr int kHalves = C::kVr == kTile ? 2 : 1, kSteps = C::kVr / 16 / kHalves;
+#pragma unroll 1
+              for (int half = 0; half < kHalves; ++half) {
+                // the first 64 keys' weights come before the others'
+                const int k0 = c * C::kVr + half * kTile / 2;
+                if (k0 == 0 || k0 == kTile / 2)
+                  ok = ok && warp_wait(&p_ready[j & 1][k0 > 0], (j >> 1) & 1);
+                tc_fence_after();
+                if (!ok) break;
+                if (k0 == 0) add = j > 0 || *(volatile int*)&s_first;
+                if (elect_one()) {
+#pragma unroll
+                  for (int k = 0; k < kSteps; ++k)
+                    umma_ts<PAIR>(tm_o, p + k0 / 2 + k * 8, v_lo + (half * kSteps + k) * 128, idesc,
+                                  k > 0 || k0 > 0 ? 1u : add);
+                  if (half == kHalves - 1) {
+                    commit<PAIR>(&v_empty[slot]);
+                    if (c == C::kVc - 1) commit<PAIR>(&pv_done[j & 1]);
+                  }
+                }
+                __syncwarp();
+              }
+              if (!ok) break;
+              chunk_next();
+            }
+          }
+        }
+      }
+      __syncwarp();
     }
-    __syncwarp();
   } else {
-    // ---- softmax: thread = row
-    const uint32_t tl = uint32_t(warp) << 21;  // this warp's TMEM lanes
-    const int tok = tid / G, g = tid % G;
-    const bool row_live = tok < per && tok < tile.n;
+    // ---- softmax: group = warps 0-3 or 4-7, thread = row
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    const int grp = warp >> 2, wq = warp & 3, row = tid & 127;
+    const uint32_t tl = uint32_t(wq) << 21;  // this warp's TMEM lanes
+    const int tok = rank * per + row / G, g = row % G;
+    const bool row_live = row / G < per && tok < tile.n;
     const int p = row_live ? tile.p0 + tok : -1;  // < 0: sees nothing
     int lo = 0, sink = 0;
     if (p >= 0) visible_keys(p, a.window, a.sinks, &lo, &sink);
     bool ok = true;
-    if (n_tiles > 0) {
-      // Q to shared memory, a warp per row; a negative scale turns its sign
-      constexpr int kLanes = D / 8;
-      const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
-      for (int r0 = warp * 32; r0 < warp * 32 + 32; r0 += 32 / kLanes) {
-        const int r = r0 + lane / kLanes, rl = lane % kLanes, rt = r / G;
-        uint4 v{0, 0, 0, 0};
-        if (rt < per && rt < tile.n) {
-          v = *reinterpret_cast<const uint4*>(a.q + (tile.t0 + rt) * a.q_stride_t +
-                                              (int64_t(h) * G + r % G) * a.q_stride_h + 8 * rl);
-          v.x ^= flip;
-          v.y ^= flip;
-          v.z ^= flip;
-          v.w ^= flip;
-        }
-        *reinterpret_cast<uint4*>(s_q + (rl >> 3) * kRows * 128 + swz128(r, rl & 7)) = v;
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&q_ready);
-    }
     // a page that is missing where some row looks: every tile is checked key by key
     bool hole = false;
     {
       const int sh = a.kv.page_shift;
       if (n_tiles > 0) {
-        for (int i = tid; i < (sink_any + (1 << sh) - 1) >> sh; i += 128)
+        for (int i = tid; i < (sink_any + (1 << sh) - 1) >> sh; i += 256)
           hole |= page_of(a.kv, tile.b, i << sh) < 0;
-        for (int i = (lo_any >> sh) + tid; i <= p_last >> sh; i += 128)
+        for (int i = (lo_any >> sh) + tid; i <= p_last >> sh; i += 256)
           hole |= page_of(a.kv, tile.b, i << sh) < 0;
       }
-      hole = softmax_any(hole);
+      hole = bar_any(1, 256, hole);
     }
     const float c2 = fabsf(a.scale) * kLog2e;
-    float m = -INFINITY, l = 0.f;  // m in units of S
-    // The product P V of tile j has ended.  Tiles alternate between two barriers: the one of
-    // tile j - 2 is known to have ended whenever tile j is asked for.
+    float m = -INFINITY, l = 0.f;  // m in units of S; l relative to m
+    // The product P V of tile j has ended.  Tiles alternate between two barriers: that of tile
+    // j - 2 is known to have ended whenever tile j is asked for.
     auto wait_pv = [&](int j) {
       ok = ok && warp_wait(&pv_done[j & 1], (j >> 1) & 1);
       tc_fence_after();
     };
     // A wait that runs out makes the warp's rows NaN; it goes on through the tiles without
-    // waiting, as the others may stand at the warps' common barrier.
-    for (int j = 0; j < n_tiles; ++j) {
-      const int k0 = tile_key(j), buf = j % C::kS;
-      const uint32_t ts = tm_s + tl + buf * kTile;
-      ok = ok && warp_wait(&s_full[buf], (j / C::kS) & 1);
-      tc_fence_after();
-      // every live row sees every key of the tile?
-      const bool edge = hole || tile.p0 < 0 || k0 + kTile - 1 > tile.p0 ||
-                        (k0 < lo_max && k0 + kTile > sink_all);
+    // waiting, as the others may stand at the groups' barriers.
+    for (int j = grp; j < n_tiles; j += 2) {
+      const int k0 = tile_key(j);
+      const int buf = j % C::kS;
+      const uint32_t ts = tm_s + tl + buf * kTile, tp = tm_p + tl + grp * 64;
+      const bool edge = edge_of(j, hole);
+      uint32_t bad = 0;  // of this warp's 32 keys
       if (edge) {
-        // S with what the row does not see at -inf, back to TMEM: a pass of its own keeps the
-        // tests out of the common path (one per element there made its code miss the
-        // instruction cache: 45 us a tile instead of 2)
-#pragma unroll 1
-        for (int c = 0; c < kTile; c += 16) {
-          uint32_t r[16];
-          tmem_ld16(ts + c, r);
-          tmem_ld_wait();
-          const int j0 = k0 + c;
-          const uint32_t off = hole && page_of(a.kv, tile.b, j0) < 0 ? 0x7fffffffu : 0u;
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int jj = j0 + e;
-            const bool see = jj <= p && (jj < sink || jj >= lo);
-            r[e] = see ? r[e] | off : 0xff800000u;
-          }
-          tmem_st16(ts + c, r);
-        }
-        tmem_st_wait();
-      }
-      float top = -INFINITY;
-#pragma unroll
-      for (int c = 0; c < kTile; c += 32) {
-        uint32_t r[32];
-        tmem_ld32(ts + c, r);
-        tmem_ld_wait();
-#pragma unroll
-        for (int e = 0; e < 32; ++e) top = fmaxf(top, __uint_as_float(r[e]));
-      }
-      // the maximum follows when it lags by more than kGrow (always from -inf)
-      const bool grow = (top - m) * c2 > kGrow || (m == -INFINITY && top > -INFINITY);
-      if (__any_sync(0xffffffffu, grow)) {
-        const float old = m;
-        m = fmaxf(m, top);
-        const float keep = old == -INFINITY ? 0.f : ex2((old - m) * c2);
-        l *= keep;
-        if (j > 0) {
-          wait_pv(j - 1);
-#pragma unroll 1
-          for (int d = 0; d < D; d += 16) {
-            uint32_t r[16];
-            tmem_ld16(tm_o + tl + d, r);
-            tmem_ld_wait();
-#pragma unroll
-            for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * keep);
-            tmem_st16(tm_o + tl + d, r);
-          }
-        }
-      }
-      const float base = m == -INFINITY ? 0.f : m * c2;
-#pragma unroll
-      for (int c = 0; c < kTile; c += 32) {
-        uint32_t r[32], w[16];
-        tmem_ld32(ts + c, r);
-        tmem_ld_wait();
-#pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-          const float p0 = ex2(fmaf(__uint_as_float(r[e]), c2, -base));
-          const float p1 = ex2(fmaf(__uint_as_float(r[e + 1]), c2, -base));
-          l += p0 + p1;
-          w[e / 2] = pack_bf16(p0, p1);
-        }
-        tmem_st16(ts + c / 2, w);  // over columns that have been read
-      }
-      tmem_st_wait();
-      if (edge) {
-        // V of this tile: thread = key
-        const int vseq = C::kS == 2 ? C::kKc + (j + 1 < n_tiles ? C::kKc : 0) + j * (C::kKc + C::kVc)
-                                    : C::kKc + j * (C::kKc + C::kVc);
-        const int q = vseq + tid / C::kVr, s = q % C::kSlots;
-        for (int c = 0; c < C::kVc && ok; ++c)
-          ok = warp_wait(&full[(vseq + c) % C::kSlots], ((vseq + c) / C::kSlots) & 1);
-        char* row = s_ring + s * kChunk + (tid % C::kVr) * 128;
-        const int jj = k0 + tid;
-        const bool seen = jj <= p_last && (jj < sink_any || jj >= lo_any);
-        bool bad = false;
-        if (ok && seen)
+        // V rows of this tile that somebody sees and that are not finite; a warp has 32 keys,
+        // D/8 lanes a row.  (From global memory: a pair's CTAs hold half the dims each.)
+        constexpr int kLanes = D / 8, kAt = 32 / kLanes;
 #pragma unroll 4
-          for (int i = 0; i < D / 8; ++i) {  // 16-byte pieces, each lane from its own bank on
-            const uint4 v = *reinterpret_cast<const uint4*>(row + (i >> 3) * C::kVr * 128 + (((i + lane) & 7) << 4));
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t x2 = (&v.x)[e];
-              bad |= (x2 & 0x7f80u) == 0x7f80u || (x2 & 0x7f800000u) == 0x7f800000u;
+        for (int i = 0; i < 32; i += kAt) {
+          const int jj = k0 + wq * 32 + i + lane / kLanes;
+          bool is = false;
+          if (jj <= p_last && (jj < sink_any || jj >= lo_any)) {
+            const int page = page_of(a.kv, tile.b, jj);
+            if (page >= 0) {
+              const uint4 v = *reinterpret_cast<const uint4*>(
+                  a.kv.v + page * a.kv.v_page_stride +
+                  ((int64_t(h) << a.kv.page_shift) + (jj & ((1 << a.kv.page_shift) - 1))) * D +
+                  8 * (lane % kLanes));
+              is = nonfinite2(v.x) || nonfinite2(v.y) || nonfinite2(v.z) || nonfinite2(v.w);
             }
           }
-        if (ok && (!seen || bad)) {
-          for (int i = 0; i < D / 8; ++i)
-            *reinterpret_cast<uint4*>(row + (i >> 3) * C::kVr * 128 + (((i + lane) & 7) << 4)) = uint4{0, 0, 0, 0};
+          const uint32_t who = __ballot_sync(0xffffffffu, is);
+#pragma unroll
+          for (int k = 0; k < kAt; ++k)
+            if (who >> (k * kLanes) & (kLanes == 32 ? 0xffffffffu : (1u << kLanes % 32) - 1)) bad |= 1u << (i + k);
         }
+      }
+      ok = ok && warp_wait(&s_full[grp], (j >> 1) & 1);
+      tc_fence_after();
+      uint32_t r[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld32(ts + c * 32, r[c]);
+      tmem_ld_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) tmem_signal<PAIR>(&s_free[buf]);
+      if (edge) {
+        // What the row does not see at -inf, a missing page's keys at NaN.  (In a block of its
+        // own: a test per element in the common path made its code miss the instruction cache.)
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          const uint32_t off = hole && page_of(a.kv, tile.b, k0 + c * 16) < 0 ? 0x7fffffffu : 0u;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int jj = k0 + c * 16 + e;
+            uint32_t& x = r[c >> 1][(c & 1) * 16 + e];
+            x = jj <= p && (jj < sink || jj >= lo) ? x | off : 0xff800000u;
+          }
+        }
+      }
+      float top;
+      {
+        float t[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[e] = __uint_as_float(r[0][e]);
+#pragma unroll
+        for (int e = 4; e < 128; ++e) t[e & 3] = fmaxf(t[e & 3], __uint_as_float(r[e >> 5][e & 31]));
+        top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+      }
+      // the maximum as the other group left it; it follows the tile's when it lags by more
+      // than kGrow (always from -inf)
+      float m_now = -INFINITY;
+      if (j > 0) {
+        named_bar_sync(2 + grp, 256);
+        m_now = s_m[row];
+      }
+      const bool grow = (top - m_now) * c2 > kGrow || (m_now == -INFINITY && top > -INFINITY);
+      const bool grows = __any_sync(0xffffffffu, grow);
+      const float m_was = m_now;
+      if (grows) {
+        m_now = fmaxf(m_now, top);
+        s_m[row] = m_now;
+      }
+      if (j == 0) s_m[row] = m_now;
+      if (j + 1 < n_tiles) bar_arrive(3 - grp, 256);
+      if (j >= 2) wait_pv(j - 2);  // this group's P buffer is free
+      if (grows && j > 0) {
+        const float keep = m_was == -INFINITY ? 0.f : ex2((m_was - m_now) * c2);
+        wait_pv(j - 1);
+#pragma unroll 1
+        for (int d = 0; d < D; d += 16) {
+          uint32_t x[16];
+          tmem_ld16(tm_o + tl + d, x);
+          tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * keep);
+          tmem_st16(tm_o + tl + d, x);
+        }
+      }
+      if (m != m_now) {  // this group's sum follows, whichever group moved the maximum
+        l *= m == -INFINITY ? 0.f : ex2((m - m_now) * c2);
+        m = m_now;
+      }
+      const float base = m == -INFINITY ? 0.f : m * c2;
+      const float2 cc = make_float2(c2, c2), bb = make_float2(-base, -base);
+      float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t w[16];
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          float2 y = fma2(make_float2(__uint_as_float(r[c][e]), __uint_as_float(r[c][e + 1])), cc, bb);
+          y.x = ex2(y.x);
+          y.y = ex2(y.y);
+          sum = add2(sum, y);
+          w[e / 2] = pack_bf16(y.x, y.y);
+        }
+        tmem_st16(tp + c * 16, w);
+        if (c == 1 && !edge) {
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) tmem_signal<PAIR>(&p_ready[grp][0]);
+        }
+      }
+      l += sum.x + sum.y;
+      tmem_st_wait();
+      if (edge) {
+        // Clean V of this tile: thread = key.  (With tile j - 1's product ended, the slots' uses
+        // before this one have landed, so the barriers' parity is this use's.)
+        if (j > 0) wait_pv(j - 1);
+        const int vseq = j * C::kVc, q = vseq + row / C::kVr;
+        for (int c = 0; c < C::kVc; ++c)
+          ok = ok && warp_wait(&v_local[(vseq + c) % C::kSlots], ((vseq + c) / C::kSlots) & 1);
+        char* vrow = s_v + (q % C::kSlots) * kChunk + (row % C::kVr) * 128;
+        const int jj = k0 + row;
+        const bool seen = jj <= p_last && (jj < sink_any || jj >= lo_any);
+        if (ok && (!seen || (bad >> lane & 1)))
+          for (int i = 0; i < C::kVg * 8; ++i)
+            *reinterpret_cast<uint4*>(vrow + (i >> 3) * C::kVr * 128 + (((i + lane) & 7) << 4)) = uint4{0, 0, 0, 0};
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        const uint32_t some = __ballot_sync(0xffffffffu, bad);
-        if (lane == 0) s_bad[warp] = some;
-        if (softmax_any(bad)) {
+        if (lane == 0) {
+          s_bad[grp][2 * wq] = uint16_t(bad);
+          s_bad[grp][2 * wq + 1] = uint16_t(bad >> 16);
+        }
+        if (bar_any(4 + grp, 128, bad != 0)) {
           // add these keys to the rows that see them, before the tile's product
-          if (j > 0) wait_pv(j - 1);
           if (j == 0) {
             const uint32_t zero[16] = {};
             for (int d = 0; d < D; d += 16) tmem_st16(tm_o + tl + d, zero);
             tmem_st_wait();
-            if (tid == 0) *(volatile int*)&s_first = 1;
+            if (row == 0) *(volatile int*)&s_first = 1;
           }
-          for (int w = 0; w < 4 && ok; ++w) {
-            uint32_t left = s_bad[w];
+          for (int w = 0; w < 8 && ok; ++w) {
+            uint32_t left = s_bad[grp][w];
             while (left) {
-              const int key = w * 32 + __ffs(left) - 1;
+              const int key = w * 16 + __ffs(left) - 1;
               left &= left - 1;
-              const uint32_t pw = tmem_ld1(ts + key / 2);
+              const uint32_t pw = tmem_ld1(tp + key / 2);
               tmem_ld_wait();
               const float pk = __uint_as_float(key & 1 ? pw & 0xffff0000u : pw << 16);
               const int jk = k0 + key;
@@ -493,59 +715,121 @@ __global__ void __launch_bounds__(192, Cfg<D>::kCtas) attn_prefill_kernel(
               tmem_st_wait();
             }
           }
-          softmax_any(false);  // s_bad is free again
+          bar_any(4 + grp, 128, false);  // s_bad is free again
         }
       }
-      tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_ready[buf]);
+      if (lane == 0) {
+        if (edge) {  // V in shared memory has been written too
+          mbar_arrive_cluster(mapa_shared(smem_u32(&p_ready[grp][0]), 0));
+          mbar_arrive_cluster(mapa_shared(smem_u32(&p_ready[grp][1]), 0));
+        } else {
+          tmem_signal<PAIR>(&p_ready[grp][1]);
+        }
+      }
     }
+    if (n_tiles > 1) wait_pv(n_tiles - 2);
     if (n_tiles > 0) wait_pv(n_tiles - 1);
-    // ---- epilogue: O / l
-    __nv_bfloat16* out = a.out + (int64_t(tile.t0 + tok) * a.Hq + int64_t(h) * G + g) * D;
-    const bool zero = p < 0 || n_tiles == 0;
-    const float inv = 1.f / l;
+    // ---- the groups' sums, each brought to the last maximum
+    named_bar_sync(1, 256);
+    const float m_end = n_tiles > 0 ? s_m[row] : -INFINITY;
+    s_l[grp][row] = l * (m == m_end ? 1.f : m == -INFINITY ? 0.f : ex2((m - m_end) * c2));
+    named_bar_sync(1, 256);
+    const float total = s_l[0][row] + s_l[1][row];
+    // ---- epilogue: O / l, half the dims each
+    const bool zero = p < 0, lost = tile.over || !ok;
+    const int d0 = grp * (D / 2);
+    if (gridDim.y > 1) {
+      const int64_t part = int64_t(blockIdx.x) * gridDim.y + blockIdx.y;
+      const Parts parts = parts_of(ws, int64_t(gridDim.x) * gridDim.y, D);
+      if (row_live && grp == 0)
+        parts.ml[part * kRows + row] = make_float2(m_end == -INFINITY ? -INFINITY : m_end * c2, lost ? NAN : total);
+      float* out = parts.o + (part * kRows + row) * D;
 #pragma unroll 1
-    for (int d = 0; d < D; d += 16) {
-      uint32_t r[16];
-      if (n_tiles > 0) {
+      for (int d = d0; d < d0 + D / 2 && n_tiles > 0; d += 16) {
+        uint32_t r[16];
         tmem_ld16(tm_o + tl + d, r);
         tmem_ld_wait();
-      }
-      if (row_live) {
-        uint4 y[2];
-        uint32_t* w = reinterpret_cast<uint32_t*>(y);
+        if (row_live)
 #pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-          float y0 = 0.f, y1 = 0.f;
-          if (tile.over || !ok) {
-            y0 = y1 = NAN;
-          } else if (!zero) {
-            y0 = __uint_as_float(r[e]) * inv;
-            y1 = __uint_as_float(r[e + 1]) * inv;
-          }
-          w[e / 2] = pack_bf16(y0, y1);
+          for (int e = 0; e < 16; e += 4)
+            *reinterpret_cast<uint4*>(out + d + e) = uint4{r[e], r[e + 1], r[e + 2], r[e + 3]};
+      }
+    } else {
+      __nv_bfloat16* out = a.out + (int64_t(tile.t0 + tok) * a.Hq + int64_t(h) * G + g) * D;
+      const float inv = 1.f / total;
+#pragma unroll 1
+      for (int d = d0; d < d0 + D / 2; d += 16) {
+        uint32_t r[16];
+        if (n_tiles > 0) {
+          tmem_ld16(tm_o + tl + d, r);
+          tmem_ld_wait();
         }
-        reinterpret_cast<uint4*>(out + d)[0] = y[0];
-        reinterpret_cast<uint4*>(out + d)[1] = y[1];
+        if (row_live) {
+          uint4 y[2];
+          uint32_t* w = reinterpret_cast<uint32_t*>(y);
+#pragma unroll
+          for (int e = 0; e < 16; e += 2) {
+            float y0 = 0.f, y1 = 0.f;
+            if (lost) {
+              y0 = y1 = NAN;
+            } else if (!zero) {
+              y0 = __uint_as_float(r[e]) * inv;
+              y1 = __uint_as_float(r[e + 1]) * inv;
+            }
+            w[e / 2] = pack_bf16(y0, y1);
+          }
+          reinterpret_cast<uint4*>(out + d)[0] = y[0];
+          reinterpret_cast<uint4*>(out + d)[1] = y[1];
+        }
       }
     }
     tc_fence_before();
   }
-  __syncthreads();
-  if (warp == 5) tmem_dealloc(s_tmem, C::kCols);
+  zero_rows(a);
+  if (PAIR) {
+    __syncwarp();
+    cluster_sync_all();  // no CTA leaves while its peer may still signal it
+    if (warp == 10) tmem_dealloc_pair(s_tmem, 512);
+  } else {
+    __syncthreads();
+    if (warp == 10) tmem_dealloc(s_tmem, 512);
+  }
 }
 
-// Rows behind the last sequence (and before the first) get zeros.
-__global__ void __launch_bounds__(256) tail_rows_kernel(const AttnArgs a) {
-  const int64_t row = int64_t(a.Hq) * a.kv.D / 8;  // 16-byte pieces of a packed row
-  const int lo = max(a.cu_q[0], 0), hi = max(a.cu_q[a.kv.B], lo);
-  uint4* out = reinterpret_cast<uint4*>(a.out);
-  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < int64_t(min(lo, a.T)) * row; i += int64_t(gridDim.x) * 256)
-    out[i] = uint4{0, 0, 0, 0};
-  for (int64_t i = min(hi, a.T) * row + int64_t(blockIdx.x) * 256 + threadIdx.x; i < a.T * row; i += int64_t(gridDim.x) * 256)
-    out[i] = uint4{0, 0, 0, 0};
+// Joins the parts of a split call: a warp per row of a block, D/32 dims a lane.
+template <int D>
+__global__ void __launch_bounds__(256) join_kernel(const AttnArgs a, void* ws, int splits) {
+  const int G = a.Hq / a.kv.Hkv, per = kRows / G, lane = threadIdx.x & 31;
+  const int block = blockIdx.x, h = block % a.kv.Hkv;
+  const int x = int(gridDim.x) / a.kv.Hkv - 1 - block / a.kv.Hkv;
+  TileOf tile;
+  const bool any = find_tile(a, per, x, &tile);
+  pdl_wait();
+  if (!any) return;
+  const Parts parts = parts_of(ws, int64_t(gridDim.x) * splits, D);
+  for (int row = blockIdx.y * 8 + (threadIdx.x >> 5); row < tile.n * G; row += gridDim.y * 8) {
+    const int tok = row / G, p = tile.p0 + tok;
+    const int64_t at = (int64_t(block) * splits * kRows + row);
+    float top = -INFINITY;
+    for (int s = 0; s < splits; ++s) top = fmaxf(top, parts.ml[at + int64_t(s) * kRows].x);
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, acc[D / 32] = {};
+    for (int s = 0; s < splits; ++s) {
+      const float2 ml = parts.ml[at + int64_t(s) * kRows];
+      if (ml.x == -INFINITY && ml.y == 0.f) continue;  // no key there: its O may be unwritten
+      const float f = ex2(ml.x - base);
+      sum += ml.y * (ml.x == -INFINITY ? 1.f : f);
+#pragma unroll
+      for (int e = 0; e < D / 32; ++e)
+        acc[e] += f * parts.o[(at + int64_t(s) * kRows) * D + lane + 32 * e];
+    }
+    __nv_bfloat16* out = a.out + (int64_t(tile.t0 + tok) * a.Hq + int64_t(h) * G + row % G) * D;
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e)
+      out[lane + 32 * e] = __float2bfloat16_rn(tile.over ? NAN : p < 0 ? 0.f : acc[e] / sum);
+  }
 }
 
 bool page_map(CUtensorMap* map, const PagedKV& kv, const __nv_bfloat16* base, int64_t page_stride,
@@ -553,47 +837,95 @@ bool page_map(CUtensorMap* map, const PagedKV& kv, const __nv_bfloat16* base, in
   const uint64_t D = kv.D, ps = uint64_t(1) << kv.page_shift;
   const uint64_t dims[5] = {64, ps, D / 64, uint64_t(kv.Hkv), uint64_t(kv.n_pages)};
   const uint64_t strides[4] = {D * 2, 128, ps * D * 2, uint64_t(page_stride) * 2};
-  const uint32_t box[5] = {64, uint32_t(rows), 1, 1, 1};
+  const uint32_t box[5] = {64, ps < uint64_t(rows) ? uint32_t(ps) : uint32_t(rows), 1, 1, 1};
   return make_tmap_bf16_nd(map, base, 5, dims, strides, box);
 }
 
-template <int D>
-cudaError_t launch_one(const AttnArgs& a, cudaStream_t st) {
-  using C = Cfg<D>;
-  const int ps = 1 << a.kv.page_shift, per = kRows / (a.Hq / a.kv.Hkv);
-  CUtensorMap mk{}, mv{};
-  if (a.kv.max_pages > 0 &&
-      (!page_map(&mk, a.kv, a.kv.k, a.kv.k_page_stride, ps < kTile ? ps : kTile) ||
-       !page_map(&mv, a.kv, a.kv.v, a.kv.v_page_stride, ps < C::kVr ? ps : C::kVr)))
+// How a call runs: rows in pairs of CTAs, or in single CTAs, which may split the keys.
+struct Plan {
+  bool pair;
+  int splits;
+  int64_t slots;  // of find_tile
+};
+Plan plan_of(int T, int B, int Hq, int Hkv, int D, int64_t keys) {
+  const int per = kRows / (Hq / Hkv);
+  const int64_t slots = int64_t(T) / per + B;
+  const int64_t tiles = int64_t(T) / per > B ? int64_t(T) / per : B;  // about what is there
+  // few rows: enough CTAs for the GPU, two tiles of keys each at least
+  int64_t splits = 148 / (tiles * Hkv);
+  if (splits > keys / (2 * kTile)) splits = keys / (2 * kTile);
+  if (splits > 1) return {false, int(splits), slots};
+  const bool pair = D >= 128 && int64_t(T) / per >= 2 * int64_t(B);
+  return {pair, 1, pair ? int64_t(T) / (2 * per) + B : slots};
+}
+
+template <int D, bool PAIR>
+cudaError_t launch_one(const AttnArgs& a, const Plan& plan, void* ws, cudaStream_t st) {
+  using C = Cfg<D, PAIR>;
+  CUtensorMap mq{}, mk{}, mv{};
+  const uint32_t G = uint32_t(a.Hq / a.kv.Hkv);
+  const uint64_t q_dims[3] = {uint64_t(D), uint64_t(a.Hq), uint64_t(a.T)};
+  const uint64_t q_strides[2] = {uint64_t(a.Hq > 1 ? a.q_stride_h : D) * 2,
+                                 uint64_t(a.T > 1 ? a.q_stride_t : int64_t(a.Hq) * D) * 2};
+  const uint32_t q_box[3] = {64, G, kRows / G};
+  if (!make_tmap_bf16_nd(&mq, a.q, 3, q_dims, q_strides, q_box)) return cudaErrorInvalidValue;
+  if (a.kv.max_pages > 0 && (!page_map(&mk, a.kv, a.kv.k, a.kv.k_page_stride, C::kKr) ||
+                             !page_map(&mv, a.kv, a.kv.v, a.kv.v_page_stride, C::kVr)))
     return cudaErrorInvalidValue;
-  const int64_t tiles = int64_t(a.T) / per + a.kv.B;  // slots of find_tile
-  if (tiles * a.kv.Hkv > 0x7fffffffLL) return cudaErrorInvalidValue;
-  attn_prefill_kernel<D><<<unsigned(tiles * a.kv.Hkv), 192, C::kSmem, st>>>(mk, mv, a);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  tail_rows_kernel<<<16, 256, 0, st>>>(a);
-  return cudaGetLastError();
+  const int64_t blocks = plan.slots * a.kv.Hkv;
+  if (blocks * C::kN > 0x7fffffffLL) return cudaErrorInvalidValue;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(blocks * C::kN), unsigned(plan.splits));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {unsigned(C::kN), 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = PAIR ? 1 : 0;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, attn_prefill_kernel<D, PAIR>, mq, mk, mv, a, ws);
+  if (e != cudaSuccess || plan.splits == 1) return e;
+  cfg.gridDim = dim3(unsigned(blocks), 4);
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = 0;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, join_kernel<D>, a, ws, plan.splits);
+}
+
+template <int D, bool PAIR> cudaError_t init_one() {
+  return cudaFuncSetAttribute(attn_prefill_kernel<D, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              Cfg<D, PAIR>::kSmem);
 }
 
 }  // namespace
 
 cudaError_t attn_prefill_init() {
-  cudaError_t e = cudaFuncSetAttribute(attn_prefill_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<64>::kSmem);
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(attn_prefill_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<128>::kSmem);
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(attn_prefill_kernel<256>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<256>::kSmem);
-  return e;
+  cudaError_t e;
+  if ((e = init_one<64, false>()) != cudaSuccess || (e = init_one<128, false>()) != cudaSuccess ||
+      (e = init_one<256, false>()) != cudaSuccess || (e = init_one<128, true>()) != cudaSuccess ||
+      (e = init_one<256, true>()) != cudaSuccess)
+    return e;
+  return cudaSuccess;
 }
 
-cudaError_t launch_attn_prefill(const AttnArgs& args, cudaStream_t st) {
+size_t attn_prefill_ws_bytes(int T, int B, int Hq, int Hkv, int D, int64_t keys) {
+  const Plan p = plan_of(T, B, Hq, Hkv, D, keys);
+  return p.splits == 1 ? 0 : size_t(p.slots) * Hkv * p.splits * kRows * (D + 2) * sizeof(float);
+}
+
+cudaError_t launch_attn_prefill(const AttnArgs& args, void* ws, cudaStream_t st) {
   AttnArgs a = args;
   if (a.T == 0) return cudaSuccess;
+  const Plan p = plan_of(a.T, a.kv.B, a.Hq, a.kv.Hkv, a.kv.D,
+                         int64_t(a.kv.max_pages) << a.kv.page_shift);
   if (a.kv.n_pages == 0) a.kv.max_pages = 0;  // no page: every row with keys gets NaN
   switch (a.kv.D) {
-    case 64: return launch_one<64>(a, st);
-    case 128: return launch_one<128>(a, st);
-    default: return launch_one<256>(a, st);
+    case 64: return launch_one<64, false>(a, p, ws, st);
+    case 128: return p.pair ? launch_one<128, true>(a, p, ws, st) : launch_one<128, false>(a, p, ws, st);
+    default: return p.pair ? launch_one<256, true>(a, p, ws, st) : launch_one<256, false>(a, p, ws, st);
   }
 }
 

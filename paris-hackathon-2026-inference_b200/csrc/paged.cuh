@@ -103,7 +103,8 @@ constexpr int kDecodeCtas = 148;
 cudaError_t launch_rope_append(const RopeArgs& a, cudaStream_t st);
 cudaError_t attn_decode_init();
 cudaError_t attn_prefill_init();
-cudaError_t launch_attn_prefill(const AttnArgs& a, cudaStream_t st);
+cudaError_t launch_attn_prefill(const AttnArgs& a, void* ws, cudaStream_t st);
+size_t attn_prefill_ws_bytes(int T, int B, int Hq, int Hkv, int D, int64_t keys);
 cudaError_t launch_attn_decode(const AttnArgs& a, void* ws, cudaStream_t st);
 size_t attn_decode_ws_bytes(int B, int Hq, int Hkv, int D);
 cudaError_t launch_pages_grow(const Pool& p, const int32_t* slots, const int32_t* add, int n,

@@ -406,10 +406,15 @@ Tensor attn_prefill_cuda(const Tensor& q, const Tensor& k_pages, const Tensor& v
   const int32_t* cu = check_cu(op, cu_q, c, q);
   const c10::cuda::CUDAGuard guard(q.device());
   Tensor out = at::empty({T, Hq, c.D}, q.options());
+  size_t nbytes = 0;
+  PMOE_CALL(pmoe_attn_prefill_workspace, T, c.B, Hq, c.Hkv, c.D, c.page_size, c.max_pages, &nbytes);
+  Tensor ws;
+  if (nbytes > 0) ws = at::empty({int64_t(nbytes)}, q.options().dtype(at::kByte));
   PMOE_CALL(pmoe_attn_prefill, bf(q), stride_of(q, 0), stride_of(q, 1), T, Hq, c.Hkv, c.D,
             bf(k_pages), bf(v_pages), c.k_stride, c.v_stride, c.n_pages, c.page_size,
             i32(page_table), c.table_stride, c.max_pages, i32(kv_lens), cu, c.B, float(scale),
-            to_int(op, "window", window), to_int(op, "sinks", sinks), bf_mut(out), stream_of(q));
+            to_int(op, "window", window), to_int(op, "sinks", sinks), bf_mut(out),
+            nbytes > 0 ? ws.data_ptr() : nullptr, nbytes, stream_of(q));
   return out;
 }
 Tensor attn_prefill_meta(const Tensor& q, const Tensor&, const Tensor&, const Tensor&,

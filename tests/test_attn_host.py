@@ -104,7 +104,7 @@ def decode(lib, q=A, st=256, sh=256, B=2, Hq=4, Hkv=2, D=128, k=A, v=A, ks=4096,
 def prefill(lib, q=A, st=256, sh=256, T=5, Hq=4, Hkv=2, D=128, ps=16, cu=A, B=2, window=0, sinks=0,
             mp=4, out=A):
     return lib.pmoe_attn_prefill(q, st, sh, T, Hq, Hkv, D, A, A, 1 << 20, 1 << 20, 8, ps, A, 4, mp,
-                                 A, cu, B, 1.0, window, sinks, out, None)
+                                 A, cu, B, 1.0, window, sinks, out, A, 1 << 30, None)
 
 
 def rope(lib, T=2, B=2, D=128, rot=32, axes=3, sec=(6, 5, 5), st=256, cu=None, pos=A, q=A, ps=16,
@@ -118,7 +118,7 @@ def rope(lib, T=2, B=2, D=128, rot=32, axes=3, sec=(6, 5, 5), st=256, cu=None, p
 @pytest.mark.parametrize("bad,status", [
     (dict(B=-1), -1), (dict(Hq=5), -1), (dict(Hkv=0), -1), (dict(D=96), -5), (dict(ps=24), -5),
     (dict(ps=8), -5), (dict(ks=100), -1), (dict(ks=4100), -2), (dict(st=12), -2),
-    (dict(sh=-8), -2), (dict(window=-1), -1), (dict(sinks=-1), -1), (dict(ts=3), -1),
+    (dict(sh=-8), -2), (dict(st=0), -2), (dict(window=-1), -1), (dict(sinks=-1), -1), (dict(ts=3), -1),
     (dict(q=None), -1), (dict(out=None), -1), (dict(lens=None), -1), (dict(table=None), -1),
     (dict(q=P(0x10008)), -2), (dict(k=P(0x10002)), -2), (dict(lens=P(0x10001)), -2),
     (dict(Hq=2 * 129), -5), (dict(mp=1 << 28, ts=1 << 28), -5), (dict(n=-1), -1)])

@@ -176,6 +176,14 @@ def test_prefill_one_long_prompt():
     check_prefill([700], [0], 16, 2, 256, 16)
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_prefill_many_rows(D):
+    """Enough tiles to fill the GPU: whole keys per CTA, in pairs of CTAs where D allows."""
+    check_prefill([700, 1, 33, 250], [0, 3, 500, 130], 16, 1, D, 16)
+    check_prefill([301, 222], [40, 0], 32, 1, D, 64, window=100, sinks=7, pad=8)
+    check_prefill([9] * 20 + [40] * 3, [300] * 23, 100, 1, D, 32)
+
+
 def test_prefill_many_short_sequences_and_rows_behind_the_last():
     check_prefill([i % 7 for i in range(70)], [(i * 11) % 50 for i in range(70)], 8, 2, 128, 16,
                   behind=13)
@@ -195,9 +203,9 @@ def test_prefill_rows_before_the_cache_get_zeros():
     R.within(got, want, bound)
 
 
-@pytest.mark.parametrize("D", [64, 256])
+@pytest.mark.parametrize("D,Hq", [(64, 2), (256, 2), (64, 64), (128, 64), (256, 64)])
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
-def test_prefill_nonfinite_keys_and_values_stay_behind_the_mask(D, bad):
+def test_prefill_nonfinite_keys_and_values_stay_behind_the_mask(D, Hq, bad):
     """A non-finite key or value changes the rows that see it and no other row."""
     from paris_moe_b200 import ops
     new, ctx, window, sinks = [100, 40], [60, 0], 37, 3
@@ -212,7 +220,7 @@ def test_prefill_nonfinite_keys_and_values_stay_behind_the_mask(D, bad):
                     pages[p, 0, 0, 0, j % 16, 3] = bad
                 if where in ("v", "both"):
                     pages[p, 0, 1, 0, j % 16, 5] = bad
-            q, cu = rand_q(140, 2, D), cu_of(new)
+            q, cu = rand_q(140, Hq, D), cu_of(new)
             args = (table, n, cu, 0.1, win, snk)
             got = ops.attn_prefill(q, pages[:, 0, 0], pages[:, 0, 1], *args).cpu()
             want, bound = R.attention(q, pages[:, 0, 0], pages[:, 0, 1], *args)

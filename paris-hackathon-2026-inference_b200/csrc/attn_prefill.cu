@@ -240,9 +240,10 @@ __device__ __forceinline__ bool find_tile(const AttnArgs& a, int per, int x, Til
   return true;
 }
 
-// Rows of no sequence get zeros (all blocks of the grid share them).
-__device__ __forceinline__ void zero_rows(const AttnArgs& a) {
-  const int lo = min(max(a.cu_q[0], 0), a.T), hi = min(max(a.cu_q[a.kv.B], lo), a.T);
+// Rows of no sequence, before cu_q[0] and from cu_q[B] on, get zeros (all blocks of the grid
+// share them).
+__device__ __forceinline__ void zero_rows(const AttnArgs& a, int first, int end) {
+  const int lo = min(max(first, 0), a.T), hi = min(max(end, lo), a.T);
   if (lo == 0 && hi == a.T) return;
   const int64_t row = int64_t(a.Hq) * a.kv.D / 8;  // 16-byte pieces of a packed row
   const int64_t id = (int64_t(blockIdx.y) * gridDim.x + blockIdx.x) * kThreads + threadIdx.x;
@@ -291,9 +292,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(
   const int block = blockIdx.x / C::kN, blocks = gridDim.x / C::kN;
   const int h = block % a.kv.Hkv;
   const int x = blocks / a.kv.Hkv - 1 - block / a.kv.Hkv;  // late tiles, the longest, first
+  const int cu_first = a.cu_q[0], cu_end = a.cu_q[a.kv.B];
   TileOf tile;
   if (!find_tile(a, per * C::kN, x, &tile)) {  // both CTAs of a pair, or none
-    zero_rows(a);
+    zero_rows(a, cu_first, cu_end);
     return;
   }
 
@@ -550,27 +552,35 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(
       const bool edge = edge_of(j, hole);
       uint32_t bad = 0;  // of this warp's 32 keys
       if (edge) {
-        // V rows of this tile that somebody sees and that are not finite; a warp has 32 keys,
-        // D/8 lanes a row.  (From global memory: a pair's CTAs hold half the dims each.)
+        // V rows of this tile that some rows see and others do not, and that are not finite; a
+        // warp has 32 keys, D/8 lanes a row.  (From global memory: a pair's CTAs hold half the
+        // dims each.  All loads at once: one latency.)
         constexpr int kLanes = D / 8, kAt = 32 / kLanes;
-#pragma unroll 4
-        for (int i = 0; i < 32; i += kAt) {
-          const int jj = k0 + wq * 32 + i + lane / kLanes;
-          bool is = false;
-          if (jj <= p_last && (jj < sink_any || jj >= lo_any)) {
-            const int page = page_of(a.kv, tile.b, jj);
-            if (page >= 0) {
-              const uint4 v = *reinterpret_cast<const uint4*>(
-                  a.kv.v + page * a.kv.v_page_stride +
-                  ((int64_t(h) << a.kv.page_shift) + (jj & ((1 << a.kv.page_shift) - 1))) * D +
-                  8 * (lane % kLanes));
-              is = nonfinite2(v.x) || nonfinite2(v.y) || nonfinite2(v.z) || nonfinite2(v.w);
-            }
-          }
-          const uint32_t who = __ballot_sync(0xffffffffu, is);
+        const int j0 = k0 + wq * 32;  // two runs of 16 keys, each within a page
+        const int pages[2] = {page_of(a.kv, tile.b, j0), page_of(a.kv, tile.b, j0 + 16)};
 #pragma unroll
-          for (int k = 0; k < kAt; ++k)
-            if (who >> (k * kLanes) & (kLanes == 32 ? 0xffffffffu : (1u << kLanes % 32) - 1)) bad |= 1u << (i + k);
+        for (int half = 0; half < 2; ++half) {
+          const __nv_bfloat16* v0 = a.kv.v + max(pages[half], 0) * a.kv.v_page_stride +
+                                    ((int64_t(h) << a.kv.page_shift) + ((j0 + 16 * half) & ((1 << a.kv.page_shift) - 1))) * D +
+                                    8 * (lane % kLanes);
+          uint4 v[16 / kAt];
+#pragma unroll
+          for (int i = 0; i < 16 / kAt; ++i) {
+            const int key = i * kAt + lane / kLanes, jj = j0 + 16 * half + key;
+            const bool some = jj <= p_last && (jj < sink_any || jj >= lo_any);
+            const bool all = jj <= tile.p0 && (jj >= lo_max || jj < sink_all);
+            v[i] = uint4{0, 0, 0, 0};
+            if (pages[half] >= 0 && some && !all) v[i] = *reinterpret_cast<const uint4*>(v0 + key * D);
+          }
+#pragma unroll
+          for (int i = 0; i < 16 / kAt; ++i) {
+            const uint32_t who = __ballot_sync(
+                0xffffffffu, nonfinite2(v[i].x) || nonfinite2(v[i].y) || nonfinite2(v[i].z) || nonfinite2(v[i].w));
+#pragma unroll
+            for (int k = 0; k < kAt; ++k)
+              if (who >> (k * kLanes) & (kLanes == 32 ? 0xffffffffu : (1u << kLanes % 32) - 1))
+                bad |= 1u << (16 * half + i * kAt + k);
+          }
         }
       }
       ok = ok && warp_wait(&s_full[grp], (j >> 1) & 1);
@@ -757,37 +767,33 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(
             *reinterpret_cast<uint4*>(out + d + e) = uint4{r[e], r[e + 1], r[e + 2], r[e + 3]};
       }
     } else {
-      __nv_bfloat16* out = a.out + (int64_t(tile.t0 + tok) * a.Hq + int64_t(h) * G + g) * D;
-      const float inv = 1.f / total;
-#pragma unroll 1
-      for (int d = d0; d < d0 + D / 2; d += 16) {
-        uint32_t r[16];
+      __nv_bfloat16* out = a.out + (int64_t(tile.t0 + tok) * a.Hq + int64_t(h) * G + g) * D + d0;
+      const float inv = lost ? NAN : zero ? 0.f : 1.f / total;
+#pragma unroll
+      for (int d = 0; d < D / 2; d += 32) {  // 64 bytes of a row at a time
+        uint32_t x[32];
         if (n_tiles > 0) {
-          tmem_ld16(tm_o + tl + d, r);
+          tmem_ld32(tm_o + tl + d0 + d, x);
           tmem_ld_wait();
         }
         if (row_live) {
-          uint4 y[2];
+          uint4 y[4];
           uint32_t* w = reinterpret_cast<uint32_t*>(y);
 #pragma unroll
-          for (int e = 0; e < 16; e += 2) {
-            float y0 = 0.f, y1 = 0.f;
-            if (lost) {
-              y0 = y1 = NAN;
-            } else if (!zero) {
-              y0 = __uint_as_float(r[e]) * inv;
-              y1 = __uint_as_float(r[e + 1]) * inv;
-            }
-            w[e / 2] = pack_bf16(y0, y1);
+          for (int e = 0; e < 32; e += 2) {
+            // (a row that sees nothing: 0 whatever its columns hold)
+            const float y0 = zero && !lost ? 0.f : __uint_as_float(x[e]) * inv;
+            const float y1 = zero && !lost ? 0.f : __uint_as_float(x[e + 1]) * inv;
+            w[e / 2] = pack_bf16(lost ? NAN : y0, lost ? NAN : y1);
           }
-          reinterpret_cast<uint4*>(out + d)[0] = y[0];
-          reinterpret_cast<uint4*>(out + d)[1] = y[1];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) reinterpret_cast<uint4*>(out + d)[e] = y[e];
         }
       }
     }
     tc_fence_before();
   }
-  zero_rows(a);
+  zero_rows(a, cu_first, cu_end);
   if (PAIR) {
     __syncwarp();
     cluster_sync_all();  // no CTA leaves while its peer may still signal it

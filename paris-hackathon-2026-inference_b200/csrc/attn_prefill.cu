@@ -206,6 +206,10 @@ template <bool PAIR> __device__ __forceinline__ void tmem_signal(uint64_t* bar) 
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity));
 }
+// The n lowest bits (n <= 0: none, n >= 32: all).
+__device__ __forceinline__ uint32_t low_bits(int n) {
+  return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1;
+}
 // Whether a 32-bit word holds a bf16 that is not finite.
 __device__ __forceinline__ bool nonfinite2(uint32_t x) {
   return (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u;
@@ -593,17 +597,25 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(
       __syncwarp();
       if (lane == 0) tmem_signal<PAIR>(&s_free[buf]);
       if (edge) {
-        // What the row does not see at -inf, a missing page's keys at NaN.  (In a block of its
-        // own: a test per element in the common path made its code miss the instruction cache.)
+        // What the row does not see at -inf, as bits of the tile's keys: 0..hi but not
+        // [a, b).  (A comparison per element took 7000 cycles a tile, most of it fetching code.)
+        const int hi = p - k0, ka = sink - k0, kb = lo - k0;
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          const uint32_t off = hole && page_of(a.kv, tile.b, k0 + c * 16) < 0 ? 0x7fffffffu : 0u;
+        for (int c = 0; c < 4; ++c) {
+          const uint32_t see = low_bits(hi + 1 - 32 * c) & (low_bits(ka - 32 * c) | ~low_bits(kb - 32 * c));
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int jj = k0 + c * 16 + e;
-            uint32_t& x = r[c >> 1][(c & 1) * 16 + e];
-            x = jj <= p && (jj < sink || jj >= lo) ? x | off : 0xff800000u;
-          }
+          for (int e = 0; e < 32; ++e)
+            if (!(see >> e & 1)) r[c][e] = 0xff800000u;
+        }
+        if (hole) {  // keys without a page: NaN where they are seen
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+            if (page_of(a.kv, tile.b, k0 + c * 16) < 0)
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                uint32_t& x = r[c >> 1][(c & 1) * 16 + e];
+                x = x == 0xff800000u ? x : 0x7fffffffu;
+              }
         }
       }
       float top;
@@ -631,7 +643,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(
       }
       if (j == 0) s_m[row] = m_now;
       if (j + 1 < n_tiles) bar_arrive(3 - grp, 256);
-      if (j >= 2) wait_pv(j - 2);  // this group's P buffer is free
       if (grows && j > 0) {
         const float keep = m_was == -INFINITY ? 0.f : ex2((m_was - m_now) * c2);
         wait_pv(j - 1);
@@ -663,6 +674,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(
           sum = add2(sum, y);
           w[e / 2] = pack_bf16(y.x, y.y);
         }
+        if (c == 0 && j >= 2) wait_pv(j - 2);  // this group's P buffer is free
         tmem_st16(tp + c * 16, w);
         if (c == 1 && !edge) {
           tmem_st_wait();
@@ -674,9 +686,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(
       l += sum.x + sum.y;
       tmem_st_wait();
       if (edge) {
-        // Clean V of this tile: thread = key.  (With tile j - 1's product ended, the slots' uses
-        // before this one have landed, so the barriers' parity is this use's.)
-        if (j > 0) wait_pv(j - 1);
+        // Clean V of this tile: thread = key.  The slots' uses before this one have to have landed
+        // for the barriers' parity to be this use's: they belong to tile j - 2 or before, whose
+        // product has ended, or, in a short ring, to tile j - 1.
+        if (C::kSlots < 2 * C::kVc && j > 0) wait_pv(j - 1);
         const int vseq = j * C::kVc, q = vseq + row / C::kVr;
         for (int c = 0; c < C::kVc; ++c)
           ok = ok && warp_wait(&v_local[(vseq + c) % C::kSlots], ((vseq + c) / C::kSlots) & 1);
@@ -693,6 +706,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(
         }
         if (bar_any(4 + grp, 128, bad != 0)) {
           // add these keys to the rows that see them, before the tile's product
+          if (j > 0) wait_pv(j - 1);
           if (j == 0) {
             const uint32_t zero[16] = {};
             for (int d = 0; d < D; d += 16) tmem_st16(tm_o + tl + d, zero);

@@ -9,10 +9,10 @@
 //                     the next tile's product at once, and writes P (bf16) to TMEM
 //   O += P V          A = P from TMEM, B = V from shared memory (dims contiguous), O in TMEM
 // Two groups of four softmax warps take the even and the odd tiles, each with a P buffer of its
-// own, so that one group's exponentials run beside the other's maxima and beside the products.  The running maximum m
-// of a row passes from group to group through shared memory.  It moves only when a tile's
-// maximum exceeds it by more than 8 (in powers of two): weights then stay below 2^8, exact to
-// the same relative rounding, and O is rescaled rarely.
+// own, so that one group's exponentials run beside the other's maxima and beside the products.
+// The running maximum m of a row passes from group to group through shared memory.  It moves
+// only when a tile's maximum exceeds it by more than 8 (in powers of two): weights then stay
+// below 2^8, exact to the same relative rounding, and O is rescaled rarely.
 //
 // In a pair each CTA fetches half of every tile (64 of the keys of K, half the dims of V) and the
 // products read both halves (cta_group::2): a lone CTA asks for 128 KiB of K and V per 2048
@@ -221,18 +221,11 @@ struct TileOf {
   int b, t0, n, p0, len;  // sequence, first packed row, tokens, index of the first, keys
   bool over;
 };
-// (A whole warp calls this: it searches 32 places at a time.)
+// (A whole warp calls this.)
 __device__ __forceinline__ bool find_tile(const AttnArgs& a, int per, int x, TileOf* o) {
-  const int lane = threadIdx.x & 31;
-  int lo = 0, n = a.kv.B;  // the last b in [lo, lo + n) whose slots begin at or before x
-  do {
-    const int step = (n + 31) / 32, b = lo + lane * step;
-    const bool before = lane * step < n && a.cu_q[b] / per + b <= x;
-    const int k = __popc(__ballot_sync(0xffffffffu, before));
-    if (k == 0) return false;
-    n = min(step, n - (k - 1) * step);
-    lo += (k - 1) * step;
-  } while (n > 1);
+  const int32_t* cu = a.cu_q;
+  const int lo = last_at_or_before(a.kv.B, x, [=](int b) { return cu[b] / per + b; });
+  if (lo < 0) return false;
   const int c0 = a.cu_q[lo], c1 = min(a.cu_q[lo + 1], a.T), len = a.kv.kv_lens[lo];
   const int i = x - (c0 / per + lo);
   if (c0 < 0 || c1 <= c0 || i < 0 || i > (c1 - c0 - 1) / per) return false;

@@ -48,16 +48,22 @@ __host__ __device__ __forceinline__ void visible_keys(int p, int window, int sin
   *sink = sinks < *lo ? sinks : *lo;
 }
 
-// The sequence that packed row t belongs to (cu[b] <= t < cu[b+1]), or -1 behind the
-// last.  cu ascends; binary search for the last b with cu[b] <= t.
-__host__ __device__ __forceinline__ int seq_of(const int32_t* cu, int B, int t) {
-  if (t < cu[0] || t >= cu[B]) return -1;
-  int lo = 0, hi = B;  // cu[lo] <= t < cu[hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (cu[mid] <= t) lo = mid; else hi = mid;
+// The last b in [0, B) with key(b) <= x, or -1; key ascends.  32 places at a time by a whole
+// warp: one step for 32 sequences, two for 1024.
+template <typename Key>
+__device__ __forceinline__ int last_at_or_before(int B, int x, Key key) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, n = B;
+  while (n > 0) {
+    const int step = (n + 31) / 32, at = lane * step;
+    const bool before = at < n && key(lo + at) <= x;
+    const int k = __popc(__ballot_sync(0xffffffffu, before));
+    if (k == 0) return -1;
+    lo += (k - 1) * step;
+    n = step < n - (k - 1) * step ? step : n - (k - 1) * step;
+    if (step == 1) break;
   }
-  return lo;
+  return B > 0 ? lo : -1;
 }
 
 struct AttnArgs {

@@ -257,6 +257,8 @@ int64_t stride_of(const Tensor& t, int dim) { return t.size(dim) <= 1 ? 0 : t.st
 
 // Rows [T, heads, D]: any token and head stride, contiguous heads.
 void check_rows(const char* op, const char* name, const Tensor& t, const Tensor& x) {
+  TORCH_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()), "paris_moe.", op, ": ", name,
+              " requires grad, and the operator has no backward pass (call it under no_grad)");
   TORCH_CHECK(t.is_cuda(), "paris_moe.", op, ": ", name, " must be a CUDA tensor");
   TORCH_CHECK(t.device() == x.device(), "paris_moe.", op, ": ", name, " is on ", t.device(),
               ", expected ", x.device());
@@ -673,4 +675,17 @@ TORCH_LIBRARY_IMPL(paris_moe, Meta, m) {
   m.impl("pages_fork", &pages_fork_meta);
   m.impl("pages_free", &pages_free_meta);
   m.impl("pages_compact", &pages_compact_meta);
+}
+
+// The attention half serves only; its operators have no backward pass (and raise where their
+// inputs ask for one), so calls go past autograd's boxed fallback, which costs several
+// microseconds for a dozen tensors.
+TORCH_LIBRARY_IMPL(paris_moe, Autograd, m) {
+  m.impl("rope_append", torch::CppFunction::makeFallthrough());
+  m.impl("attn_decode", torch::CppFunction::makeFallthrough());
+  m.impl("attn_prefill", torch::CppFunction::makeFallthrough());
+  m.impl("pages_grow", torch::CppFunction::makeFallthrough());
+  m.impl("pages_fork", torch::CppFunction::makeFallthrough());
+  m.impl("pages_free", torch::CppFunction::makeFallthrough());
+  m.impl("pages_compact", torch::CppFunction::makeFallthrough());
 }

@@ -24,7 +24,6 @@ extern "C" int h_page_of(const int* table, long stride, int max_pages, int shift
   kv.n_pages = n_pages;
   return page_of(kv, b, j);
 }
-extern "C" int h_seq_of(const int* cu, int B, int t) { return seq_of(cu, B, t); }
 extern "C" int h_len(int len, int max_pages, int shift, int* over) {
   bool o; int r = kv_len_of(len, max_pages, shift, &o); *over = o; return r;
 }
@@ -69,13 +68,6 @@ def test_lengths_beyond_the_table_are_cut_and_reported(host):
     over = ctypes.c_int()
     for n, want, o in [(-5, 0, 0), (0, 0, 0), (48, 48, 0), (49, 48, 1), (2 ** 31 - 1, 48, 1)]:
         assert host.h_len(n, 3, 4, ctypes.byref(over)) == want and over.value == o
-
-
-@pytest.mark.parametrize("cu", [[0, 3, 3, 3, 7], [0, 0], [0, 0, 1], [2, 5, 5, 9], [0] * 5])
-def test_rows_find_their_sequence(host, cu):
-    for t in range(-1, 11):
-        want = next((b for b in range(len(cu) - 1) if cu[b] <= t < cu[b + 1]), -1)
-        assert host.h_seq_of(ints(cu), len(cu) - 1, t) == want
 
 
 def test_visible_keys(host):

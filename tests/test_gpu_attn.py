@@ -318,6 +318,11 @@ def test_bad_arguments_raise():
         ops.attn_prefill(q, k, v, table, n, cu_of([1]), 0.1)
     with pytest.raises(RuntimeError, match="16-byte"):
         ops.attn_decode(rand_q(2, 4, 68)[..., 4:], k, v, table, n, 0.1)
+    grad = q.clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="no backward pass"):
+        ops.attn_decode(grad, k, v, table, n, 0.1)
+    with torch.no_grad():
+        assert torch.equal(ops.attn_decode(grad, k, v, table, n, 0.1), ops.attn_decode(q, k, v, table, n, 0.1))
 
 
 # ---- rotary positions and the cache write -------------------------------------------------

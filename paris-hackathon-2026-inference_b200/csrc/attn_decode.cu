@@ -120,20 +120,18 @@ template <int D, int NT> constexpr int decode_smem() {
          R::kWarps * 8 * NT * 2 * 4;
 }
 
-// Workspace: prefix[B+1] int64 (units before sequence b, per head group), then two
-// partial results per CTA: O [8 NT][D], then (m, l) [8 NT][2], in 32 bits.
+// Workspace: two partial results per CTA, O [8 NT][D], then (m, l) [8 NT][2], in 32 bits; then
+// the first and the last CTA of every item.
 struct DecodeWs {
-  int64_t* prefix;
   float* o;
   float* ml;
+  int* ctas;  // [items][2]
 };
-__host__ __device__ inline DecodeWs decode_ws(void* ws, int B, int heads, int D) {
-  char* p = static_cast<char*>(ws);
+__host__ __device__ inline DecodeWs decode_ws(void* ws, int heads, int D) {
   DecodeWs w;
-  w.prefix = reinterpret_cast<int64_t*>(p);
-  p += (size_t(B) + 1) * 8 + 15 & ~size_t(15);
-  w.o = reinterpret_cast<float*>(p);
+  w.o = static_cast<float*>(ws);
   w.ml = w.o + size_t(2) * kDecodeCtas * heads * D;
+  w.ctas = reinterpret_cast<int*>(w.ml + size_t(2) * kDecodeCtas * heads * 2);
   return w;
 }
 
@@ -170,7 +168,8 @@ __global__ void __launch_bounds__(Ring<D>::kWarps * 32, 1) attn_decode_kernel(
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int G = a.Hq / a.kv.Hkv, chunks = (G + GH - 1) / GH, Hc = a.kv.Hkv * chunks;
-  const DecodeWs ws = decode_ws(ws_raw, a.kv.B, GH, D);
+  const DecodeWs ws = decode_ws(ws_raw, GH, D);
+  pdl_trigger();  // combine_kernel's CTAs may take their places and wait
 
   // ---- the plan: units per sequence, summed over the block --------------------
   const int per = (a.kv.B + kThreads - 1) / kThreads;
@@ -202,16 +201,11 @@ __global__ void __launch_bounds__(Ring<D>::kWarps * 32, 1) attn_decode_kernel(
   }
   const int64_t U = total * Hc;
   const int n = active_ctas(U, n_items * Hc, W);
-  if (blockIdx.x == 0) {  // for combine_kernel
-    int64_t at = before;
-    for (int b = b_lo; b < b_hi; ++b) {
-      ws.prefix[b] = at;
-      at += seq_geo(a, b).units;
-    }
-    if (tid == 0) ws.prefix[a.kv.B] = total;
-  }
   if (int(blockIdx.x) >= n) return;
-  const int64_t u0 = int64_t(blockIdx.x) * U / n, u1 = int64_t(blockIdx.x + 1) * U / n;
+  // equal pieces, the first U % n of them one longer
+  const int64_t whole = U <= 0x7fffffff ? int64_t(int(U) / n) : U / n;
+  const int more = int(U - whole * n), c = blockIdx.x;
+  const int64_t u0 = c * whole + min(c, more), u1 = u0 + whole + (c < more);
   if (before * Hc <= u0 && u0 < (before + mine) * Hc) {
     int64_t at = before;
     int b = b_lo;
@@ -425,7 +419,10 @@ __global__ void __launch_bounds__(Ring<D>::kWarps * 32, 1) attn_decode_kernel(
           o[d][t][c + 2] *= f;
         }
       }
-    const bool whole = at == item0 && end == item1;
+    const bool alone = at == item0 && end == item1;
+    const int64_t item = int64_t(seg.b) * Hc + seg.hc;
+    if (tid == 0 && at == item0) ws.ctas[item * 2] = blockIdx.x;
+    if (tid == 0 && end == item1) ws.ctas[item * 2 + 1] = blockIdx.x;
     const int part = int(blockIdx.x) * 2 + (at == item0 ? 1 : 0);
 #pragma unroll
     for (int d0 = 0; d0 < D; d0 += kJoinDims) {
@@ -443,7 +440,7 @@ __global__ void __launch_bounds__(Ring<D>::kWarps * 32, 1) attn_decode_kernel(
         float acc = 0.f;
 #pragma unroll
         for (int w = 0; w < W; ++w) acc += s_join[(w * GH + g) * kJoinPitch + d];
-        if (whole) {
+        if (alone) {
           if (g0 + g < G) {
             float top = -INFINITY, sum = 0.f;
             for (int w = 0; w < W; ++w) top = fmaxf(top, s_m[w * GH + g]);
@@ -458,7 +455,7 @@ __global__ void __launch_bounds__(Ring<D>::kWarps * 32, 1) attn_decode_kernel(
       }
       __syncthreads();
     }
-    if (!whole)
+    if (!alone)
       for (int g = tid; g < GH; g += kThreads) {
         float top = -INFINITY, sum = 0.f;
         for (int w = 0; w < W; ++w) top = fmaxf(top, s_m[w * GH + g]);
@@ -471,48 +468,41 @@ __global__ void __launch_bounds__(Ring<D>::kWarps * 32, 1) attn_decode_kernel(
     at = end;
     __syncthreads();  // s_m and s_l are free again
   }
-  pdl_trigger();
 }
 
 // One CTA per (sequence, query head): joins the parts of an item that several CTAs
 // computed, in CTA order, and writes the rows that have no keys.
-__global__ void __launch_bounds__(256) combine_kernel(const AttnArgs a, void* ws_raw, int GH,
-                                                      int warps) {
+__global__ void __launch_bounds__(256) combine_kernel(const AttnArgs a, void* ws_raw, int GH) {
   const int b = blockIdx.x / a.Hq, h = blockIdx.x % a.Hq, tid = threadIdx.x;
   const int D = a.kv.D, G = a.Hq / a.kv.Hkv, chunks = (G + GH - 1) / GH, Hc = a.kv.Hkv * chunks;
   const int g = h % G, hc = h / G * chunks + g / GH, gl = g % GH;
   __nv_bfloat16* out = a.out + (int64_t(b) * a.Hq + h) * D;
-  const Seq s = seq_geo(a, b);
-  if (s.units == 0) {
+  const DecodeWs ws = decode_ws(ws_raw, GH, D);
+  if (seq_geo(a, b).units == 0) {
     bool over;
     kv_len_of(a.kv.kv_lens[b], a.kv.max_pages, a.kv.page_shift, &over);
     for (int d = tid; d < D; d += 256) out[d] = __float2bfloat16_rn(over ? NAN : 0.f);
-    pdl_wait();
     return;
   }
-  __shared__ int s_items;
-  if (tid == 0) s_items = 0;
-  __syncthreads();
-  int mine = 0;
-  for (int i = tid; i < a.kv.B; i += 256) mine += seq_geo(a, i).units > 0;
-  if (mine) atomicAdd(&s_items, mine);
   pdl_wait();
-  __syncthreads();
-  const DecodeWs ws = decode_ws(ws_raw, a.kv.B, GH, D);
-  const int64_t U = ws.prefix[a.kv.B] * Hc;
-  const int n = active_ctas(U, int64_t(s_items) * Hc, warps);
-  const int64_t first = ws.prefix[b] * Hc + int64_t(hc) * s.units, last = first + s.units - 1;
-  auto cta_of = [&](int64_t u) {  // c U/n <= u < (c+1) U/n
-    int c = int(u * n / U);
-    while (int64_t(c + 1) * U / n <= u) ++c;
-    while (int64_t(c) * U / n > u) --c;
-    return c;
-  };
-  const int c0 = cta_of(first), c1 = cta_of(last);
+  const int2 range = reinterpret_cast<const int2*>(ws.ctas)[int64_t(b) * Hc + hc];
+  const int c0 = range.x, c1 = range.y;
   if (c0 == c1) return;  // written by that CTA
+  auto part_of = [&](int c) { return size_t(2 * c + (c == c0)) * GH + gl; };
+  // (m, l) of all parts, a thread each, while O is on its way
+  __shared__ float2 s_ml[kDecodeCtas];
+  __shared__ float s_top[8];
   float top = -INFINITY;
-  for (int c = c0; c <= c1; ++c)
-    top = fmaxf(top, ws.ml[(size_t(2 * c + (c == c0)) * GH + gl) * 2]);
+  if (c0 + tid <= c1) {
+    s_ml[tid] = reinterpret_cast<const float2*>(ws.ml)[part_of(c0 + tid)];
+    top = s_ml[tid].x;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if ((tid & 31) == 0) s_top[tid >> 5] = top;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 8; ++k) top = fmaxf(top, s_top[k]);
   const float base = top == -INFINITY ? 0.f : top;
   // D/4 threads of 16 bytes, the CTAs' parts dealt out over the 1024/D groups of them
   __shared__ float s_sum[16];
@@ -520,11 +510,12 @@ __global__ void __launch_bounds__(256) combine_kernel(const AttnArgs a, void* ws
   const int lanes = D / 4, group = tid / lanes, groups = 256 / lanes, d4 = tid % lanes;
   float sum = 0.f;
   float4 acc{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
   for (int c = c0 + group; c <= c1; c += groups) {
-    const size_t part = size_t(2 * c + (c == c0)) * GH + gl;
-    const float f = fast_exp2(ws.ml[part * 2] - base);
-    const float4 x = reinterpret_cast<const float4*>(ws.o + part * D)[d4];
-    sum += ws.ml[part * 2 + 1] * f;
+    const float2 ml = s_ml[c - c0];
+    const float f = fast_exp2(ml.x - base);
+    const float4 x = reinterpret_cast<const float4*>(ws.o + part_of(c) * D)[d4];
+    sum += ml.y * f;
     acc.x += x.x * f;
     acc.y += x.y * f;
     acc.z += x.z * f;
@@ -565,7 +556,7 @@ cudaError_t launch_one(const AttnArgs& a, const CUtensorMap& mk, const CUtensorM
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, combine_kernel, a, ws, 8 * NT, int(Ring<D>::kWarps));
+  return cudaLaunchKernelEx(&cfg, combine_kernel, a, ws, 8 * NT);
 }
 
 template <int D, int NT> cudaError_t init_one() {
@@ -578,8 +569,9 @@ int heads_per_item(int G) { return G <= 8 ? 8 : 16; }
 }  // namespace
 
 size_t attn_decode_ws_bytes(int B, int Hq, int Hkv, int D) {
-  const DecodeWs w = decode_ws(nullptr, B, heads_per_item(Hq / Hkv), D);
-  return reinterpret_cast<size_t>(w.ml + size_t(2) * kDecodeCtas * heads_per_item(Hq / Hkv) * 2);
+  const int heads = heads_per_item(Hq / Hkv), chunks = (Hq / Hkv + heads - 1) / heads;
+  return size_t(2) * kDecodeCtas * heads * (D + 2) * sizeof(float) +
+         size_t(B) * Hkv * chunks * 2 * sizeof(int);
 }
 
 cudaError_t attn_decode_init() {

@@ -188,6 +188,7 @@ __global__ void __launch_bounds__(Ring<D>::kWarps * 32, 1) attn_decode_kernel(
     it += z;
   }
   __shared__ int64_t s_items[W];
+  __shared__ float s_inv[GH];
   if (lane == 31) s_scan[warp] = incl, s_items[warp] = it;
   if (lane == 0)
     for (int s = 0; s < S; ++s) mbar_init(&s_bar[warp * S + s], 1);
@@ -224,37 +225,54 @@ __global__ void __launch_bounds__(Ring<D>::kWarps * 32, 1) attn_decode_kernel(
   seg.b = int(s_start[0]);
   seg.s = seq_geo(a, seg.b);
   {
-    const int64_t off = u0 - s_start[1];
-    seg.hc = int(off / seg.s.units);
-    seg.k = int(off - int64_t(seg.hc) * seg.s.units);
+    const int off = int(u0 - s_start[1]);  // (a sequence's units in all heads fit 32 bits)
+    seg.hc = off / seg.s.units;
+    seg.k = off - seg.hc * seg.s.units;
   }
-  Walk fetch = seg;
-  walk(a, Hc, fetch, warp);
-  int64_t u_fetch = u0 + warp, u = u0 + warp;  // next unit to fetch, to consume
   char* ring = smem + warp * S * 2 * R::kOperand;
   uint64_t* bars = s_bar + warp * S;
+  int64_t u_fetch = u0 + warp, u = u0 + warp;  // next unit to fetch, to consume
+  // Where the warp's next 32 units to fetch lie, a lane each: one page lookup's latency for
+  // all of them.
+  Walk ahead = seg;  // at the first of the 32
+  walk(a, Hc, ahead, warp);
+  int my_page = -1, my_row = 0, my_head = 0, nth = 0;
+  auto look = [&]() {
+    Walk w = ahead;
+    my_page = -1;
+    if (u_fetch + int64_t(lane) * W < u1) {
+      walk(a, Hc, w, lane * W);
+      const int key = unit_key(w.s, w.k);
+      my_page = page_of(a.kv, w.b, key);
+      my_row = key & ((1 << a.kv.page_shift) - 1);
+      my_head = w.hc / chunks;
+    }
+  };
+  look();
   uint32_t bad = 0;  // slots whose unit lies in no page
   int slot_f = 0, slot_c = 0, phase_c = 0, in_flight = 0;
   bool dead = false;
-  int page = u_fetch < u1 ? page_of(a.kv, fetch.b, unit_key(fetch.s, fetch.k)) : -1;
   auto fetch_one = [&]() {
     if (u_fetch >= u1 || dead) return;
+    if (nth == 32) {
+      walk(a, Hc, ahead, 32 * W);
+      look();
+      nth = 0;
+    }
+    const int page = __shfl_sync(0xffffffffu, my_page, nth), row = __shfl_sync(0xffffffffu, my_row, nth);
+    const int h = __shfl_sync(0xffffffffu, my_head, nth);
     bad = page < 0 ? bad | 1u << slot_f : bad & ~(1u << slot_f);
     if (lane == 0) {
-      const int row = unit_key(fetch.s, fetch.k) & ((1 << a.kv.page_shift) - 1);
       const uint32_t dst = smem_u32(ring + slot_f * 2 * R::kOperand);
-      const int h = fetch.hc / chunks, at = page < 0 ? a.kv.n_pages : page;  // no page: zeros
+      const int at = page < 0 ? a.kv.n_pages : page;  // no page: zeros
       mbar_arrive_expect_tx(&bars[slot_f], 2 * R::kOperand);
       tma_load_5d(dst, &map_k, row, h, at, &bars[slot_f]);
       tma_load_5d(dst + R::kOperand, &map_v, row, h, at, &bars[slot_f]);
     }
     slot_f = slot_f + 1 == S ? 0 : slot_f + 1;
     ++in_flight;
+    ++nth;
     u_fetch += W;
-    if (u_fetch < u1) {  // the next unit's page, long before it is needed
-      walk(a, Hc, fetch, W);
-      page = page_of(a.kv, fetch.b, unit_key(fetch.s, fetch.k));
-    }
   };
   for (int s = 0; s < S; ++s) fetch_one();
 
@@ -292,7 +310,7 @@ __global__ void __launch_bounds__(Ring<D>::kWarps * 32, 1) attn_decode_kernel(
       // a wait that runs out makes the rows NaN and stops the fetching; what is in flight
       // is still waited for
       if (in_flight > 0) {
-        if (!mbar_wait(&bars[slot_c], phase_c)) dead = true;
+        if (!__all_sync(0xffffffffu, mbar_wait(&bars[slot_c], phase_c))) dead = true;
         --in_flight;
       }
       const int j0 = unit_key(seg.s, int(u - item0));
@@ -424,46 +442,59 @@ __global__ void __launch_bounds__(Ring<D>::kWarps * 32, 1) attn_decode_kernel(
     if (tid == 0 && at == item0) ws.ctas[item * 2] = blockIdx.x;
     if (tid == 0 && end == item1) ws.ctas[item * 2 + 1] = blockIdx.x;
     const int part = int(blockIdx.x) * 2 + (at == item0 ? 1 : 0);
+    // The sum over the warps of dims d0 .. d0 + n - 1, which lie in buf [W][GH][n + 4].
+    auto add_up = [&](const float* buf, int d0, int n) {
+      for (int i = tid; i < GH * n; i += kThreads) {
+        const int g = i / n, d = i % n;
+        float acc = 0.f;
 #pragma unroll
-    for (int d0 = 0; d0 < D; d0 += kJoinDims) {
+        for (int w = 0; w < W; ++w) acc += buf[(w * GH + g) * (n + 4) + d];
+        if (!alone) {
+          ws.o[(size_t(part) * GH + g) * D + d0 + d] = acc;
+        } else if (g0 + g < G) {
+          a.out[(int64_t(seg.b) * a.Hq + int64_t(h_kv) * G + g0 + g) * D + d0 + d] =
+              __float2bfloat16_rn(acc * s_inv[g]);
+        }
+      }
+    };
+    if (tid < GH) {  // 1 / l of the joined heads
+      float top = -INFINITY, sum = 0.f;
+      for (int w = 0; w < W; ++w) top = fmaxf(top, s_m[w * GH + tid]);
+      for (int w = 0; w < W; ++w)
+        sum += s_l[w * GH + tid] * fast_exp2(s_m[w * GH + tid] - (top == -INFINITY ? 0.f : top));
+      s_inv[tid] = 1.f / sum;
+      if (!alone) {
+        ws.ml[(size_t(part) * GH + tid) * 2] = top;
+        ws.ml[(size_t(part) * GH + tid) * 2 + 1] = sum;
+      }
+    }
+    if (end == u1) {  // nothing is on its way any more: all dims at once, in the ring
+      float* buf = reinterpret_cast<float*>(smem);
 #pragma unroll
-      for (int dd = 0; dd < kJoinDims / 16; ++dd)
+      for (int d = 0; d < D / 16; ++d)
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            s_join[(warp * GH + t * 8 + (lane & 3) * 2 + (e & 1)) * kJoinPitch + dd * 16 +
-                   (lane >> 2) + 8 * (e >> 1)] = o[d0 / 16 + dd][t][e];
+            buf[(warp * GH + t * 8 + (lane & 3) * 2 + (e & 1)) * (D + 4) + d * 16 + (lane >> 2) + 8 * (e >> 1)] = o[d][t][e];
       __syncthreads();
-      for (int i = tid; i < GH * kJoinDims; i += kThreads) {
-        const int g = i / kJoinDims, d = i % kJoinDims;
-        float acc = 0.f;
+      add_up(buf, 0, D);
+    } else {
 #pragma unroll
-        for (int w = 0; w < W; ++w) acc += s_join[(w * GH + g) * kJoinPitch + d];
-        if (alone) {
-          if (g0 + g < G) {
-            float top = -INFINITY, sum = 0.f;
-            for (int w = 0; w < W; ++w) top = fmaxf(top, s_m[w * GH + g]);
-            for (int w = 0; w < W; ++w)
-              sum += s_l[w * GH + g] * fast_exp2(s_m[w * GH + g] - (top == -INFINITY ? 0.f : top));
-            a.out[(int64_t(seg.b) * a.Hq + int64_t(h_kv) * G + g0 + g) * D + d0 + d] =
-                __float2bfloat16_rn(acc / sum);
-          }
-        } else {
-          ws.o[(size_t(part) * GH + g) * D + d0 + d] = acc;
-        }
+      for (int d0 = 0; d0 < D; d0 += kJoinDims) {
+#pragma unroll
+        for (int dd = 0; dd < kJoinDims / 16; ++dd)
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              s_join[(warp * GH + t * 8 + (lane & 3) * 2 + (e & 1)) * kJoinPitch + dd * 16 +
+                     (lane >> 2) + 8 * (e >> 1)] = o[d0 / 16 + dd][t][e];
+        __syncthreads();
+        add_up(s_join, d0, kJoinDims);
+        __syncthreads();
       }
-      __syncthreads();
     }
-    if (!alone)
-      for (int g = tid; g < GH; g += kThreads) {
-        float top = -INFINITY, sum = 0.f;
-        for (int w = 0; w < W; ++w) top = fmaxf(top, s_m[w * GH + g]);
-        for (int w = 0; w < W; ++w)
-          sum += s_l[w * GH + g] * fast_exp2(s_m[w * GH + g] - (top == -INFINITY ? 0.f : top));
-        ws.ml[(size_t(part) * GH + g) * 2] = top;
-        ws.ml[(size_t(part) * GH + g) * 2 + 1] = sum;
-      }
     walk(a, Hc, seg, int(end - at));
     at = end;
     __syncthreads();  // s_m and s_l are free again

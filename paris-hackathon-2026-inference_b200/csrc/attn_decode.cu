@@ -22,6 +22,8 @@
 // Bound by HBM: each visible key and value is read once.  64 sequences of up to 16384 keys
 // (1.107 GB): 188 us, 5.9 TB/s, 91 % of the copy rate.  192 KiB of slots per SM keep about
 // 160 KiB in flight; one box per operand and unit, as a unit never leaves its page.
+#include <algorithm>
+
 #include "paged.cuh"
 #include "pmoe_tma.cuh"
 
@@ -171,6 +173,11 @@ __global__ void __launch_bounds__(Ring<D>::kWarps * 32, 1) attn_decode_kernel(
   const DecodeWs ws = decode_ws(ws_raw, GH, D);
   pdl_trigger();  // combine_kernel's CTAs may take their places and wait
 
+  if (lane == 0)
+    for (int s = 0; s < S; ++s) mbar_init(&s_bar[warp * S + s], 1);
+  mbar_fence_init();
+  pdl_wait();
+
   // ---- the plan: units per sequence, summed over the block --------------------
   const int per = (a.kv.B + kThreads - 1) / kThreads;
   const int b_lo = min(a.kv.B, tid * per), b_hi = min(a.kv.B, b_lo + per);
@@ -190,9 +197,6 @@ __global__ void __launch_bounds__(Ring<D>::kWarps * 32, 1) attn_decode_kernel(
   __shared__ int64_t s_items[W];
   __shared__ float s_inv[GH];
   if (lane == 31) s_scan[warp] = incl, s_items[warp] = it;
-  if (lane == 0)
-    for (int s = 0; s < S; ++s) mbar_init(&s_bar[warp * S + s], 1);
-  mbar_fence_init();
   __syncthreads();
   int64_t before = incl - mine, total = 0, n_items = 0;
   for (int w = 0; w < W; ++w) {
@@ -509,13 +513,16 @@ __global__ void __launch_bounds__(256) combine_kernel(const AttnArgs a, void* ws
   const int g = h % G, hc = h / G * chunks + g / GH, gl = g % GH;
   __nv_bfloat16* out = a.out + (int64_t(b) * a.Hq + h) * D;
   const DecodeWs ws = decode_ws(ws_raw, GH, D);
-  if (seq_geo(a, b).units == 0) {
+  // (kv_lens is older than the main kernel, which has waited for whatever wrote it)
+  const int len = a.kv.kv_lens[b];
+  const bool none = seq_geo(a, b).units == 0;
+  pdl_wait();
+  if (none) {
     bool over;
-    kv_len_of(a.kv.kv_lens[b], a.kv.max_pages, a.kv.page_shift, &over);
+    kv_len_of(len, a.kv.max_pages, a.kv.page_shift, &over);
     for (int d = tid; d < D; d += 256) out[d] = __float2bfloat16_rn(over ? NAN : 0.f);
     return;
   }
-  pdl_wait();
   const int2 range = reinterpret_cast<const int2*>(ws.ctas)[int64_t(b) * Hc + hc];
   const int c0 = range.x, c1 = range.y;
   if (c0 == c1) return;  // written by that CTA
@@ -574,20 +581,15 @@ __global__ void __launch_bounds__(256) combine_kernel(const AttnArgs a, void* ws
 template <int D, int NT>
 cudaError_t launch_one(const AttnArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, void* ws,
                        cudaStream_t st) {
-  attn_decode_kernel<D, NT><<<kDecodeCtas, Ring<D>::kWarps * 32, decode_smem<D, NT>(), st>>>(
-      mk, mv, a, ws);
-  cudaError_t e = cudaGetLastError();
+  // no more CTAs than the tables' width leaves work for
+  const int G = a.Hq / a.kv.Hkv, chunks = (G + 8 * NT - 1) / (8 * NT);
+  const int64_t items = int64_t(a.kv.B) * a.kv.Hkv * chunks;
+  const int64_t units = (int64_t(a.kv.max_pages) << a.kv.page_shift) / kUnit * items;
+  const int64_t most = std::max((units + Ring<D>::kWarps - 1) / Ring<D>::kWarps, items);
+  cudaError_t e = launch_dependent(attn_decode_kernel<D, NT>, dim3(unsigned(std::min<int64_t>(most, kDecodeCtas))),
+                                   Ring<D>::kWarps * 32, decode_smem<D, NT>(), 1, st, mk, mv, a, ws);
   if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(a.kv.B) * a.Hq);
-  cfg.blockDim = dim3(256);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, combine_kernel, a, ws, 8 * NT);
+  return launch_dependent(combine_kernel, dim3(unsigned(a.kv.B) * a.Hq), 256, 0, 1, st, a, ws, 8 * NT);
 }
 
 template <int D, int NT> cudaError_t init_one() {

@@ -289,6 +289,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(
   const int block = blockIdx.x / C::kN, blocks = gridDim.x / C::kN;
   const int h = block % a.kv.Hkv;
   const int x = blocks / a.kv.Hkv - 1 - block / a.kv.Hkv;  // late tiles, the longest, first
+  pdl_wait();
+  pdl_trigger();
   const int cu_first = a.cu_q[0], cu_end = a.cu_q[a.kv.B];
   TileOf tile;
   if (!find_tile(a, per * C::kN, x, &tile)) {  // both CTAs of a pair, or none
@@ -887,25 +889,11 @@ cudaError_t launch_one(const AttnArgs& a, const Plan& plan, void* ws, cudaStream
     return cudaErrorInvalidValue;
   const int64_t blocks = plan.slots * a.kv.Hkv;
   if (blocks * C::kN > 0x7fffffffLL) return cudaErrorInvalidValue;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(blocks * C::kN), unsigned(plan.splits));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = C::kSmem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim = {unsigned(C::kN), 1, 1};
-  cfg.attrs = attr;
-  cfg.numAttrs = PAIR ? 1 : 0;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, attn_prefill_kernel<D, PAIR>, mq, mk, mv, a, ws);
+  cudaError_t e = launch_dependent(attn_prefill_kernel<D, PAIR>,
+                                   dim3(unsigned(blocks * C::kN), unsigned(plan.splits)), kThreads,
+                                   C::kSmem, C::kN, st, mq, mk, mv, a, ws);
   if (e != cudaSuccess || plan.splits == 1) return e;
-  cfg.gridDim = dim3(unsigned(blocks), 4);
-  cfg.blockDim = dim3(256);
-  cfg.dynamicSmemBytes = 0;
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, join_kernel<D>, a, ws, plan.splits);
+  return launch_dependent(join_kernel<D>, dim3(unsigned(blocks), 4), 256, 0, 1, st, a, ws, plan.splits);
 }
 
 template <int D, bool PAIR> cudaError_t init_one() {

@@ -106,6 +106,28 @@ struct Pool {
 // CTAs of the decode kernel: one per SM of a B200.
 constexpr int kDecodeCtas = 148;
 
+// Launch with programmatic stream serialisation: the kernel's set-up may run while its
+// predecessor in the stream ends.  Every kernel launched this way waits (griddepcontrol.wait)
+// before it reads or writes anything that the predecessor might still use, on all its paths, so
+// that a kernel behind it may rely on everything before it.
+template <typename... KArgs, typename... Args>
+cudaError_t launch_dependent(void (*kernel)(KArgs...), dim3 grid, unsigned block, size_t smem,
+                             unsigned cluster, cudaStream_t st, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim = {cluster, 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 cudaError_t launch_rope_append(const RopeArgs& a, cudaStream_t st);
 cudaError_t attn_decode_init();
 cudaError_t attn_prefill_init();

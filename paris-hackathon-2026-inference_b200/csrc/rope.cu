@@ -6,6 +6,7 @@
 // The angle is formed and reduced to (-pi, pi] in 64 bits: at position 1e6 a 32-bit
 // product is already off by 0.03 rad.  One rounding to bf16, at the store.
 #include "paged.cuh"
+#include "pmoe_tma.cuh"
 
 namespace pmoe {
 
@@ -62,6 +63,7 @@ __global__ void __launch_bounds__(kRopeThreads, 4) rope_append_kernel(const Rope
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int t = (blockIdx.x * kWarps + warp) / S, part = warp % S;
   if (t >= a.T) return;  // (a whole warp)
+  pdl_wait();
   const int rl = lane % kLanes, sub = lane / kLanes;  // this lane's 8 dims 8*rl .., row of a slot
   // Rows r0, r0 + step, .. of q, then of k, then of v are this lane's.
   const int r0 = part * kRows + sub, step = S * kRows;
@@ -200,8 +202,8 @@ __global__ void __launch_bounds__(kRopeThreads, 4) rope_append_kernel(const Rope
 template <int D, int S>
 cudaError_t launch_split(const RopeArgs& a, cudaStream_t st) {
   const int64_t warps = int64_t(a.T) * S, per = kRopeThreads / 32;
-  rope_append_kernel<D, S><<<unsigned((warps + per - 1) / per), kRopeThreads, 0, st>>>(a);
-  return cudaGetLastError();
+  return launch_dependent(rope_append_kernel<D, S>, dim3(unsigned((warps + per - 1) / per)),
+                          kRopeThreads, 0, 1, st, a);
 }
 
 template <int D>

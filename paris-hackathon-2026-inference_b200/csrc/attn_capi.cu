@@ -104,7 +104,7 @@ int make_pool(Pool* p, uint16_t* pages, int n_pages, int chunks, int page_size, 
               int32_t* lens, bool need_lens) {
   if (n_pages < 0 || max_pages < 0 || S < 0 || (S > 1 && table_stride < max_pages))
     return PMOE_ERR_ARG;
-  if (page_shift_of(page_size) < 0) return PMOE_ERR_UNSUPPORTED;
+  if (page_shift_of(page_size) < 0 || n_pages > 1 << 29) return PMOE_ERR_UNSUPPORTED;
   if (int64_t(max_pages) * page_size > 0x7fff0000LL) return PMOE_ERR_UNSUPPORTED;
   if ((n_pages > 0 && !refs) || (S > 0 && need_lens && !lens) ||
       (S > 0 && max_pages > 0 && !tables))

@@ -3,6 +3,7 @@
 // tables and the lengths; the free pages are those with refs 0, handed out lowest number
 // first, so the same calls give the same pages on every run.
 #include "paged.cuh"
+#include "pmoe_tma.cuh"
 
 namespace pmoe {
 
@@ -11,13 +12,15 @@ namespace {
 constexpr int kPlanThreads = 1024;
 constexpr int kPerThread = 4;
 
-// Inclusive scan of x over the block; *total gets the sum.
+// Inclusive scan of x >= 0 over the block; *total gets the sum.  Sums stop at kMost, above any
+// number of pages.
+constexpr int kMost = 0x3fffffff;
 __device__ __forceinline__ int block_scan(int x, int* s_warp, int* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
+    if (lane >= o) x = min(x + y, kMost);
   }
   __syncthreads();  // s_warp of the scan before has been read
   if (lane == 31) s_warp[warp] = x;
@@ -26,36 +29,65 @@ __device__ __forceinline__ int block_scan(int x, int* s_warp, int* total) {
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int y = __shfl_up_sync(0xffffffffu, w, o);
-    if (lane >= o) w += y;
+    if (lane >= o) w = min(w + y, kMost);
   }
   *total = __shfl_sync(0xffffffffu, w, 31);
   const int before = __shfl_sync(0xffffffffu, w, warp == 0 ? 0 : warp - 1);
-  return x + (warp == 0 ? 0 : before);
+  return min(x + (warp == 0 ? 0 : before), kMost);
+}
+
+// The free pages among 4 * kPlanThreads refs, a thread's four loaded beforehand.
+struct Refs4 {
+  int r[kPerThread];
+};
+__device__ __forceinline__ Refs4 load_refs(const int32_t* refs, int n_pages, int p0) {
+  Refs4 x;
+  const int p = p0 + threadIdx.x * kPerThread;
+#pragma unroll
+  for (int k = 0; k < kPerThread; ++k) x.r[k] = p + k < n_pages ? refs[p + k] : 1;
+  return x;
 }
 
 // The first `want` free pages in ascending order into pick; returns how many there were.
-__device__ __forceinline__ int pick_free(const int32_t* refs, int n_pages, int want,
+// `first`: the refs of the pages 0 .. 4095, which the caller loads while it does other things.
+__device__ __forceinline__ int pick_free(const int32_t* refs, int n_pages, int want, Refs4 first,
                                          int32_t* pick, int* s_warp) {
   int found = 0;
   for (int p0 = 0; p0 < n_pages && found < want; p0 += kPlanThreads * kPerThread) {
+    const Refs4 x = p0 == 0 ? first : load_refs(refs, n_pages, p0);
     const int p = p0 + threadIdx.x * kPerThread;
-    bool open[kPerThread];
     int mine = 0, total;
 #pragma unroll
-    for (int k = 0; k < kPerThread; ++k) {
-      open[k] = p + k < n_pages && refs[p + k] == 0;
-      mine += open[k];
-    }
+    for (int k = 0; k < kPerThread; ++k) mine += x.r[k] == 0;
     int at = found + block_scan(mine, s_warp, &total) - mine;
 #pragma unroll
     for (int k = 0; k < kPerThread; ++k)
-      if (open[k]) {
+      if (x.r[k] == 0) {
         if (at < want) pick[at] = p + k;
         ++at;
       }
     found += total;
   }
   return min(found, want);
+}
+
+// Room in shared memory for the marks of so many sequences and for the requests of one round;
+// more go through the workspace.
+constexpr int kMarks = 4096, kRequests = kPlanThreads;
+
+// What a request asks for: pages (-1: refused), and the number asked for up to and with it.
+struct Requests {
+  int32_t *need, *end, *pick;
+};
+struct PlanSmem {
+  int warp[32], mark[kMarks], need[kRequests], end[kRequests];
+};
+__device__ __forceinline__ Requests requests_of(PlanSmem& s, int32_t* ws, int n) {
+  Requests q;
+  q.need = n <= kRequests ? s.need : ws;
+  q.end = n <= kRequests ? s.end : ws + n;
+  q.pick = ws + 2 * size_t(n);
+  return q;
 }
 
 // mark[slot] = the first request that names the slot.
@@ -67,98 +99,101 @@ __device__ __forceinline__ void mark_first(int32_t* mark, int S, const int32_t* 
   __syncthreads();
 }
 
-__global__ void __launch_bounds__(kPlanThreads) pages_grow_kernel(
-    const Pool p, const int32_t* slots, const int32_t* add, int n, int32_t* ok, int32_t* ws) {
-  __shared__ int s_warp[32];
-  int32_t *mark = ws, *need = mark + p.S, *end = need + n, *pick = end + n;
-  const int tid = threadIdx.x, ps = 1 << p.page_shift;
-  mark_first(mark, p.S, slots, n);
+// Requests in order: need[i] = ask(i) pages, end[i] their running sum; returns how many pages
+// there are for them.  A request is granted if need >= 0 and end <= that.
+template <typename Ask>
+__device__ __forceinline__ int serve(const Pool& p, int n, Refs4 first, PlanSmem& sm, Requests q, Ask ask) {
   int64_t carry = 0;
   for (int i0 = 0; i0 < n; i0 += kPlanThreads) {
-    const int i = i0 + tid;
-    int want = -1;  // -1: refused
-    if (i < n) {
-      const int s = slots[i];
-      if (s >= 0 && s < p.S && mark[s] == i && add[i] >= 0) {
-        const int64_t old = p.lens[s], len = old + add[i];
-        if (old >= 0 && len <= int64_t(p.max_pages) << p.page_shift && len <= 0x7fffffff)
-          want = int(((len + ps - 1) >> p.page_shift) - ((old + ps - 1) >> p.page_shift));
-      }
-    }
+    const int i = i0 + threadIdx.x;
+    const int want = i < n ? ask(i) : -1;
     int total;
-    const int64_t e = carry + block_scan(max(want, 0), s_warp, &total);
+    const int64_t e = carry + block_scan(max(want, 0), sm.warp, &total);
     if (i < n) {
-      need[i] = want;
-      end[i] = int(min(e, int64_t(p.n_pages) + 1));  // beyond the pool: granted to nobody
+      q.need[i] = want;
+      q.end[i] = int(min(e, int64_t(p.n_pages) + 1));  // beyond the pool: granted to nobody
     }
     carry += total;
   }
+  const int found = pick_free(p.refs, p.n_pages, int(min(carry, int64_t(p.n_pages))), first, q.pick, sm.warp);
   __syncthreads();
-  const int found = pick_free(p.refs, p.n_pages, int(min(carry, int64_t(p.n_pages))), pick, s_warp);
-  __syncthreads();
-  const int lane = tid & 31;
-  for (int i = tid >> 5; i < n; i += kPlanThreads / 32) {
-    const int want = need[i], e = end[i], s = slots[i];
-    const bool yes = want >= 0 && e <= found;
-    if (yes) {
-      const int old = p.lens[s], first = int((int64_t(old) + ps - 1) >> p.page_shift);
-      for (int j = lane; j < want; j += 32) {
-        const int page = pick[e - want + j];
-        p.tables[s * p.table_stride + first + j] = page;
-        p.refs[page] = 1;
-      }
-      __syncwarp();
-      if (lane == 0) p.lens[s] = old + add[i];
+  return found;
+}
+
+// ws: mark[S], need[n], end[n], pick[n_pages]
+__global__ void __launch_bounds__(kPlanThreads) pages_grow_kernel(
+    const Pool p, const int32_t* slots, const int32_t* add, int n, int32_t* ok, int32_t* ws) {
+  __shared__ PlanSmem sm;
+  const int tid = threadIdx.x, ps = 1 << p.page_shift;
+  pdl_wait();
+  const Refs4 first = load_refs(p.refs, p.n_pages, 0);
+  int32_t* mark = p.S <= kMarks ? sm.mark : ws;
+  const Requests q = requests_of(sm, ws + p.S, n);
+  mark_first(mark, p.S, slots, n);
+  const int found = serve(p, n, first, sm, q, [&](int i) {
+    const int s = slots[i], a = add[i];
+    if (s < 0 || s >= p.S || mark[s] != i || a < 0) return -1;
+    const int64_t old = p.lens[s], len = old + a;
+    if (old < 0 || len > int64_t(p.max_pages) << p.page_shift || len > 0x7fffffff) return -1;
+    return int(((len + ps - 1) >> p.page_shift) - ((old + ps - 1) >> p.page_shift));
+  });
+  // the granted pages, a thread each: page k belongs to the first request with end > k
+  for (int k = tid; k < found; k += kPlanThreads) {
+    int lo = 0, hi = n - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (q.end[mid] > k) hi = mid; else lo = mid + 1;
     }
-    if (lane == 0) ok[i] = yes;
+    if (q.end[lo] > found) continue;  // the first that did not fit
+    const int s = slots[lo], page = q.pick[k];
+    const int have = int((int64_t(p.lens[s]) + ps - 1) >> p.page_shift);
+    p.tables[s * p.table_stride + have + k - (q.end[lo] - q.need[lo])] = page;
+    p.refs[page] = 1;
+  }
+  __syncthreads();  // the lengths have been read
+  for (int i = tid; i < n; i += kPlanThreads) {
+    const bool yes = q.need[i] >= 0 && q.end[i] <= found;
+    if (yes) p.lens[slots[i]] += add[i];
+    ok[i] = yes;
   }
 }
 
-// ws: mark[S], plan[n] (fresh page, -1: none needed, -2: refused), need[n], end[n], pick
+// ws: plan[n] (fresh page, -1: none needed, -2: refused), mark[S], need[n], end[n], pick[n_pages]
 __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(
     const Pool p, const int32_t* src, const int32_t* dst, const int32_t* keep, int n,
     int32_t* ok, int32_t* ws) {
-  __shared__ int s_warp[32];
-  int32_t *mark = ws, *plan = mark + p.S, *need = plan + n, *end = need + n, *pick = end + n;
+  __shared__ PlanSmem sm;
   const int tid = threadIdx.x, ps = 1 << p.page_shift;
+  pdl_wait();
+  pdl_trigger();
+  const Refs4 first = load_refs(p.refs, p.n_pages, 0);
+  int32_t *plan = ws, *mark = p.S <= kMarks ? sm.mark : ws + n;
+  const Requests q = requests_of(sm, ws + n + p.S, n);
   mark_first(mark, p.S, dst, n);
-  int carry = 0;
-  for (int i0 = 0; i0 < n; i0 += kPlanThreads) {
-    const int i = i0 + tid;
-    int want = -1;
-    if (i < n) {
-      const int s = src[i], d = dst[i], k = keep[i];
-      // a target is empty, named once and nobody's source
-      if (s >= 0 && s < p.S && d >= 0 && d < p.S && mark[d] == i && mark[s] == 0x7fffffff &&
-          p.lens[d] == 0 && k >= 0 && k <= p.lens[s] &&
-          k <= int64_t(p.max_pages) << p.page_shift) {
-        want = 0;
-        if (k & (ps - 1)) {
-          const int t = p.tables[s * p.table_stride + (k >> p.page_shift)];
-          want = t >= 0 && t < p.n_pages;
-        }
-      }
-    }
-    int total;
-    const int e = carry + block_scan(max(want, 0), s_warp, &total);
-    if (i < n) need[i] = want, end[i] = e;
-    carry += total;
-  }
-  __syncthreads();
-  const int found = pick_free(p.refs, p.n_pages, min(carry, p.n_pages), pick, s_warp);
-  __syncthreads();
+  const int found = serve(p, n, first, sm, q, [&](int i) {
+    const int s = src[i], d = dst[i], k = keep[i];
+    // a target is empty, named once and nobody's source
+    if (s < 0 || s >= p.S || d < 0 || d >= p.S || mark[d] != i || mark[s] != 0x7fffffff || k < 0 ||
+        k > int64_t(p.max_pages) << p.page_shift)
+      return -1;
+    const int full = k >> p.page_shift;
+    const int tail = k & (ps - 1) ? p.tables[s * p.table_stride + full] : -1;
+    if (p.lens[d] != 0 || k > p.lens[s]) return -1;
+    return int(tail >= 0 && tail < p.n_pages);
+  });
   for (int i = tid; i < n; i += kPlanThreads) {
-    const bool yes = need[i] >= 0 && end[i] <= found;
+    const bool yes = q.need[i] >= 0 && q.end[i] <= found;
     ok[i] = yes;
-    plan[i] = !yes ? -2 : need[i] ? pick[end[i] - 1] : -1;
+    plan[i] = !yes ? -2 : q.need[i] ? q.pick[q.end[i] - 1] : -1;
   }
 }
 
 // gridDim = (n, parts): part 0 copies the table row, all parts copy the tail page.
 __global__ void __launch_bounds__(256) fork_copy_kernel(const Pool p, const int32_t* src,
                                                         const int32_t* dst, const int32_t* keep,
-                                                        const int32_t* plan_ws) {
-  const int i = blockIdx.x, fresh = plan_ws[p.S + i];
+                                                        const int32_t* plan) {
+  pdl_wait();
+  const int i = blockIdx.x, fresh = plan[i];
   if (fresh == -2) return;
   const int k = keep[i], full = k >> p.page_shift, used = k & ((1 << p.page_shift) - 1);
   const int32_t* from = p.tables + src[i] * p.table_stride;
@@ -182,15 +217,24 @@ __global__ void __launch_bounds__(256) fork_copy_kernel(const Pool p, const int3
   const __nv_bfloat16* s0 = p.pages + size_t(from[full]) * p.chunks * chunk;
   __nv_bfloat16* d0 = p.pages + size_t(fresh) * p.chunks * chunk;
   const int vec = used * p.D / 8;  // 16-byte pieces of a chunk's used rows
-  for (int c = blockIdx.y; c < p.chunks; c += gridDim.y) {
-    const uint4* s = reinterpret_cast<const uint4*>(s0 + c * chunk);
-    uint4* d = reinterpret_cast<uint4*>(d0 + c * chunk);
-    for (int j = threadIdx.x; j < vec; j += blockDim.x) d[j] = s[j];
-  }
+  // four chunks' pieces on their way at a time
+  constexpr int kOnce = 4;
+  for (int j = threadIdx.x; j < vec; j += blockDim.x)
+    for (int c = blockIdx.y; c < p.chunks; c += kOnce * gridDim.y) {
+      uint4 x[kOnce];
+#pragma unroll
+      for (int k = 0; k < kOnce; ++k)
+        if (c + k * int(gridDim.y) < p.chunks)
+          x[k] = reinterpret_cast<const uint4*>(s0 + (c + k * gridDim.y) * chunk)[j];
+#pragma unroll
+      for (int k = 0; k < kOnce; ++k)
+        if (c + k * int(gridDim.y) < p.chunks) reinterpret_cast<uint4*>(d0 + (c + k * gridDim.y) * chunk)[j] = x[k];
+    }
 }
 
 __global__ void __launch_bounds__(256) pages_free_kernel(const Pool p, const int32_t* slots,
                                                          int window, int sinks) {
+  pdl_wait();
   const int s = slots[blockIdx.x];
   if (s < 0 || s >= p.S) return;
   int lo = 0, hi = p.max_pages;
@@ -216,6 +260,8 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const Pool p
                                                                     int32_t* remap, int32_t* ws) {
   __shared__ int s_warp[32];
   const int tid = threadIdx.x;
+  pdl_wait();
+  pdl_trigger();
   int32_t* movers = ws + 16;
   int mine = 0, n_live;
   for (int q = tid; q < p.n_pages; q += kPlanThreads) mine += p.refs[q] > 0;
@@ -255,6 +301,7 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const Pool p
 
 __global__ void __launch_bounds__(256) compact_move_kernel(const Pool p, const int32_t* remap,
                                                            const int32_t* ws) {
+  pdl_wait();
   const int moves = ws[0];
   const int64_t entries = int64_t(p.S) * p.max_pages;
   for (int64_t e = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; e < entries;
@@ -274,7 +321,17 @@ __global__ void __launch_bounds__(256) compact_move_kernel(const Pool p, const i
     const uint4* s = reinterpret_cast<const uint4*>(p.pages) + from * page_vec;
     uint4* d = reinterpret_cast<uint4*>(p.pages) + to * page_vec;
     const size_t j0 = (w % parts) * part, j1 = min(j0 + part, page_vec);
-    for (size_t j = j0 + threadIdx.x; j < j1; j += blockDim.x) d[j] = s[j];
+    uint4 x[8];  // all of the thread's pieces on their way at once
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const size_t j = j0 + threadIdx.x + k * 256;
+      if (j < j1) x[k] = __ldcs(s + j);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const size_t j = j0 + threadIdx.x + k * 256;
+      if (j < j1) __stcs(d + j, x[k]);
+    }
   }
 }
 
@@ -283,32 +340,33 @@ __global__ void __launch_bounds__(256) compact_move_kernel(const Pool p, const i
 cudaError_t launch_pages_grow(const Pool& p, const int32_t* slots, const int32_t* add, int n,
                               int32_t* ok, int32_t* ws, cudaStream_t st) {
   if (n == 0) return cudaSuccess;
-  pages_grow_kernel<<<1, kPlanThreads, 0, st>>>(p, slots, add, n, ok, ws);
-  return cudaGetLastError();
+  return launch_dependent(pages_grow_kernel, dim3(1), kPlanThreads, 0, 1, st, p, slots, add, n, ok, ws);
 }
 
 cudaError_t launch_pages_fork(const Pool& p, const int32_t* src, const int32_t* dst,
                               const int32_t* keep, int n, int32_t* ok, int32_t* ws,
                               cudaStream_t st) {
   if (n == 0) return cudaSuccess;
-  fork_plan_kernel<<<1, kPlanThreads, 0, st>>>(p, src, dst, keep, n, ok, ws);
-  const dim3 grid(n, p.chunks < 8 ? p.chunks : 8);
-  fork_copy_kernel<<<grid, 256, 0, st>>>(p, src, dst, keep, ws);
-  return cudaGetLastError();
+  const cudaError_t e = launch_dependent(fork_plan_kernel, dim3(1), kPlanThreads, 0, 1, st, p, src, dst,
+                                         keep, n, ok, ws);
+  if (e != cudaSuccess) return e;
+  return launch_dependent(fork_copy_kernel, dim3(n, p.chunks < 8 ? p.chunks : 8), 256, 0, 1, st, p, src,
+                          dst, keep, static_cast<const int32_t*>(ws));
 }
 
 cudaError_t launch_pages_free(const Pool& p, const int32_t* slots, int n, int window, int sinks,
                               cudaStream_t st) {
   if (n == 0) return cudaSuccess;
-  pages_free_kernel<<<n, 256, 0, st>>>(p, slots, window, sinks);
-  return cudaGetLastError();
+  return launch_dependent(pages_free_kernel, dim3(n), 256, 0, 1, st, p, slots, window, sinks);
 }
 
 cudaError_t launch_pages_compact(const Pool& p, int32_t* live, int32_t* remap, int32_t* ws,
                                  cudaStream_t st) {
-  compact_plan_kernel<<<1, kPlanThreads, 0, st>>>(p, live, remap, ws);
-  compact_move_kernel<<<148 * 4, 256, 0, st>>>(p, remap, ws);
-  return cudaGetLastError();
+  const cudaError_t e = launch_dependent(compact_plan_kernel, dim3(1), kPlanThreads, 0, 1, st, p, live,
+                                         remap, ws);
+  if (e != cudaSuccess) return e;
+  return launch_dependent(compact_move_kernel, dim3(148 * 4), 256, 0, 1, st, p,
+                          static_cast<const int32_t*>(remap), static_cast<const int32_t*>(ws));
 }
 
 }  // namespace pmoe

@@ -137,6 +137,19 @@ def test_many_sequences_and_pages():
     p.check()
 
 
+def test_requests_that_add_up_to_more_than_32_bits():
+    """Sums of many huge requests do not wrap round into grants."""
+    from paris_moe_b200 import ops
+    S, width = 600, 1 << 22
+    refs, lens = torch.zeros(50, dtype=torch.int32, device=DEV), torch.zeros(S, dtype=torch.int32, device=DEV)
+    tables = torch.full((S, width), -1, dtype=torch.int32, device=DEV)
+    add = [width * 16] * S
+    add[0] = 33
+    ok = ops.pages_grow(refs, tables, lens, torch.arange(S, dtype=torch.int32, device=DEV), i32(add), 16)
+    assert ok.tolist() == [1] + [0] * (S - 1) and refs.tolist() == [1] * 3 + [0] * 47
+    assert lens.tolist() == [33] + [0] * (S - 1)
+
+
 def test_random_sessions():
     for seed in range(6):
         rng = random.Random(seed)

@@ -10,6 +10,7 @@ Public surface (mirrors the reference's engine/kernels API):
       (C++ csrc/torch_ops.cpp -> libparis_moe_torch.so, loaded by ops.py)
   torch.ops.paris_moe.rope_append / attn_decode / attn_prefill / pages_*
       (the attention half over a paged cache; kv_cache.py keeps the pages)
+  MoEStack, DecoderStack                                       (stack.py)
   EPGroup (NVLink expert parallelism; comm_handle of moe_block)  (ep.py)
   workload generators                                          (workload.py)
 """
@@ -24,7 +25,8 @@ _LAZY = {
     "block_weights": "moe", "moe_block": "ops", "moe_route": "ops",
     "rope_append": "ops", "attn_decode": "ops", "attn_prefill": "ops", "pages_grow": "ops",
     "pages_fork": "ops", "pages_free": "ops", "pages_compact": "ops",
-    "PagedKVCache": "kv_cache",
+    "PagedKVCache": "kv_cache", "MoEStack": "stack", "DecoderStack": "stack",
+    "AttentionWeights": "stack", "Step": "stack",
 }
 
 

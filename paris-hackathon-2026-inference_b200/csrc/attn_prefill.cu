@@ -536,8 +536,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(
     }
     const float c2 = fabsf(a.scale) * kLog2e;
     float m = -INFINITY, l = 0.f;  // m in units of S; l relative to m
-    // The product P V of tile j has ended.  Tiles alternate between two barriers: that of tile
-    // j - 2 is known to have ended whenever tile j is asked for.
+    // The product P V of tile j has ended.  Tiles alternate between two barriers, and a barrier's
+    // parity tells two uses apart: tile j may be asked for only once tile j - 2's product is known
+    // to have ended.  (This group waits for tile j - 2 in every tile j; products end in order.)
     auto wait_pv = [&](int j) {
       ok = ok && warp_wait(&pv_done[j & 1], (j >> 1) & 1);
       tc_fence_after();
@@ -640,6 +641,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(
       if (j + 1 < n_tiles) bar_arrive(3 - grp, 256);
       if (grows && j > 0) {
         const float keep = m_was == -INFINITY ? 0.f : ex2((m_was - m_now) * c2);
+        if (j >= 2) wait_pv(j - 2);  // (which also ends tile j - 3's, before j - 1 on its barrier)
         wait_pv(j - 1);
 #pragma unroll 1
         for (int d = 0; d < D; d += 16) {

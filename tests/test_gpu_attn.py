@@ -184,6 +184,25 @@ def test_prefill_many_rows(D):
     check_prefill([9] * 20 + [40] * 3, [300] * 23, 100, 1, D, 32)
 
 
+@pytest.mark.parametrize("Hq,Hkv,D,new,ctx", [(16, 1, 128, [500, 300], [900, 1300]), (16, 1, 256, [400], [1500]),
+                                              (2, 1, 256, [130], [1700]), (4, 4, 64, [260, 40], [800, 2000])])
+def test_prefill_maxima_that_keep_growing(Hq, Hkv, D, new, ctx):
+    """Keys get larger along the sequence, so that every tile moves most rows' maxima."""
+    from paris_moe_b200 import ops
+    lens = [a + b for a, b in zip(new, ctx)]
+    pages, table, n = make_cache(lens, Hkv, D, 32, 7, layers=1)
+    for b, m in enumerate(lens):
+        for i in range(-(-m // 32)):
+            pages[table[b, i].item(), :, 0] *= 0.2 + 0.15 * i
+    q, cu = rand_q(sum(new), Hq, D, 8), cu_of(new)
+    args = (pages[:, 0, 0], pages[:, 0, 1], table, n, cu, D ** -0.5)
+    got = ops.attn_prefill(q, *args)
+    want, bound = R.attention(q, *args)
+    R.within(got, want, bound)
+    for _ in range(30):
+        assert torch.equal(ops.attn_prefill(q, *args), got)
+
+
 def test_prefill_many_short_sequences_and_rows_behind_the_last():
     check_prefill([i % 7 for i in range(70)], [(i * 11) % 50 for i in range(70)], 8, 2, 128, 16,
                   behind=13)

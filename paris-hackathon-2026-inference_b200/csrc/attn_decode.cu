@@ -171,12 +171,13 @@ __global__ void __launch_bounds__(Ring<D>::kWarps * 32, 1) attn_decode_kernel(
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int G = a.Hq / a.kv.Hkv, chunks = (G + GH - 1) / GH, Hc = a.kv.Hkv * chunks;
   const DecodeWs ws = decode_ws(ws_raw, GH, D);
-  pdl_trigger();  // combine_kernel's CTAs may take their places and wait
 
   if (lane == 0)
     for (int s = 0; s < S; ++s) mbar_init(&s_bar[warp * S + s], 1);
   mbar_fence_init();
   pdl_wait();
+  // combine_kernel's CTAs may take their places, read kv_lens (so not before the wait) and wait
+  pdl_trigger();
 
   // ---- the plan: units per sequence, summed over the block --------------------
   const int per = (a.kv.B + kThreads - 1) / kThreads;

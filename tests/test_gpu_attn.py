@@ -307,6 +307,57 @@ def test_calls_repeat_bit_for_bit_and_replay_from_graphs():
     R.within(third[0], want, bound)
 
 
+def test_calls_follow_lengths_that_the_kernel_before_them_wrote():
+    """Back to back: bookkeeping that moves the lengths, then the calls that read them."""
+    from paris_moe_b200 import PagedKVCache, ops
+    g = torch.Generator().manual_seed(2)
+    c = PagedKVCache(200, 16, 1, 1, 64, 3, 900)
+    c.pages.copy_(torch.randn(c.pages.shape, generator=g))
+    one = torch.ones(3, dtype=torch.int32, device=DEV)
+    slots = torch.arange(3, dtype=torch.int32, device=DEV)
+    q = rand_q(3, 2, 64)
+    c.grow(slots, [1, 300, 100])
+    got, at = [], []
+    for _ in range(120):
+        c.grow(slots, one)
+        got.append(ops.attn_decode(q, c.k(0), c.v(0), c.tables, c.lens, 0.2))
+        got.append(ops.attn_prefill(q, c.k(0), c.v(0), c.tables, c.lens, cu_of([1, 1, 1]), 0.2))
+        at.append(c.lens.clone())
+    for i in (0, 1, 17, 60, 119):
+        want, bound = R.attention(q, c.k(0), c.v(0), c.tables, at[i], cu_of([1, 1, 1]), 0.2)
+        R.within(got[2 * i], want, bound)
+        R.within(got[2 * i + 1], want, bound)
+    # every step's row differs from the one before: a call on stale lengths would repeat it
+    for i in range(1, 120):
+        assert not torch.equal(got[2 * i], got[2 * i - 2])
+
+
+def test_calls_on_two_streams_at_once():
+    from paris_moe_b200 import ops
+    pages, table, n = make_cache([700, 3000, 1, 64], 2, 128, 16)
+    pages2, table2, n2 = make_cache([2500, 90], 2, 128, 64, 5)
+    q, qp = rand_q(4, 8, 128), rand_q(300, 32, 128, 5)
+    cu = cu_of([180, 120 - 30])
+    qp = qp[:270]
+
+    def left():
+        return ops.attn_decode(q, pages[:, 0, 0], pages[:, 0, 1], table, n, 0.1)
+
+    def right():
+        return ops.attn_prefill(qp, pages2[:, 1, 0], pages2[:, 1, 1], table2, n2, cu, 0.1)
+    a, b = left(), right()
+    torch.cuda.synchronize()
+    s, t = torch.cuda.Stream(), torch.cuda.Stream()
+    out = []
+    for _ in range(40):
+        with torch.cuda.stream(s):
+            out.append((left(), right()))
+        with torch.cuda.stream(t):
+            out.append((left(), right()))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, a) and torch.equal(y, b) for x, y in out)
+
+
 def test_empty_calls():
     from paris_moe_b200 import ops
     pages, table, n = make_cache([5], 1, 64, 16)

@@ -63,6 +63,7 @@ int check_cache(int Hq, int Hkv, int D, int64_t kps, int64_t vps, int n_pages, i
 PagedKV make_kv(const uint16_t* k, const uint16_t* v, int64_t kps, int64_t vps, int n_pages,
                 int page_size, int Hkv, int D, const int32_t* table, int64_t table_stride,
                 int max_pages, const int32_t* kv_lens, int B) {
+  if (n_pages <= 1) kps = vps = int64_t(Hkv) * page_size * D;  // never stepped over
   return PagedKV{const_cast<__nv_bfloat16*>(bf(k)), const_cast<__nv_bfloat16*>(bf(v)), kps, vps,
                  n_pages, page_shift_of(page_size), Hkv, D, table, table_stride, max_pages,
                  kv_lens, B};

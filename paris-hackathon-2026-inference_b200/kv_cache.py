@@ -57,7 +57,9 @@ class PagedKVCache:
     def fork(self, src, dst, keep=None) -> torch.Tensor:
         """Empty sequences ``dst`` become the first ``keep`` tokens (default: all) of ``src``."""
         src = self._list(src)
-        keep = self.lens.index_select(0, src) if keep is None else self._list(keep)
+        if keep is None:   # (the call itself refuses sources out of range)
+            keep = self.lens[src.clamp(0, self.lens.shape[0] - 1)]
+        keep = self._list(keep)
         return ops.pages_fork(self.pages, self.refs, self.tables, self.lens, src,
                               self._list(dst), keep)
 

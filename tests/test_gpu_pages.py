@@ -104,6 +104,14 @@ def test_a_source_that_is_also_a_target_is_refused():
     p.check()
 
 
+def test_fork_of_everything_refuses_sources_out_of_range():
+    from paris_moe_b200 import PagedKVCache
+    c = PagedKVCache(8, 16, 1, 1, 64, 4, 64)
+    c.grow([0], [20])
+    assert c.fork([0, -3, 4, 2 ** 31 - 1], [1, 2, 3, 3]).tolist() == [1, 0, 0, 0]
+    assert c.lens.tolist() == [20, 20, 0, 0] and int(c.refs.sum()) == 4
+
+
 def test_full_pool_and_empty_lists():
     p = Pair(5, 16, 4, 8)
     p.grow([], [])

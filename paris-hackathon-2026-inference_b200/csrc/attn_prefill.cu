@@ -28,6 +28,8 @@
 // 0 x inf is NaN: in tiles at an edge of some row's sight, V rows that nobody sees or that
 // hold a non-finite number are zeroed in shared memory, and the latter are added to the rows
 // that see them one by one.
+#include <algorithm>
+
 #include "paged.cuh"
 #include "pmoe_tc.cuh"
 
@@ -250,8 +252,8 @@ __device__ __forceinline__ void zero_rows(const AttnArgs& a, int first, int end)
   for (int64_t i = hi * row + id; i < a.T * row; i += step) out[i] = uint4{0, 0, 0, 0};
 }
 
-// Parts of a split call: O [128][D] of (block x, split y), not yet divided, then each row's
-// (m, l), m in powers of two.
+// Parts of a split call: O [D/4][128 rows][4] of (block x, split y), not yet divided (a thread
+// has a row, so rows lie side by side), then each row's (m, l), m in powers of two.
 struct Parts {
   float* o;
   float2* ml;
@@ -259,6 +261,9 @@ struct Parts {
 __host__ __device__ inline Parts parts_of(void* ws, int64_t blocks, int D) {
   float* o = static_cast<float*>(ws);
   return {o, reinterpret_cast<float2*>(o + blocks * kRows * D)};
+}
+template <int D> __device__ __forceinline__ float4* part_row(const Parts& p, int64_t part, int row) {
+  return reinterpret_cast<float4*>(p.o) + part * (kRows * D / 4) + row;
 }
 
 template <int D, bool PAIR>
@@ -290,7 +295,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(
   const int h = block % a.kv.Hkv;
   const int x = blocks / a.kv.Hkv - 1 - block / a.kv.Hkv;  // late tiles, the longest, first
   pdl_wait();
-  pdl_trigger();
   const int cu_first = a.cu_q[0], cu_end = a.cu_q[a.kv.B];
   TileOf tile;
   if (!find_tile(a, per * C::kN, x, &tile)) {  // both CTAs of a pair, or none
@@ -758,6 +762,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(
     s_l[grp][row] = l * (m == m_end ? 1.f : m == -INFINITY ? 0.f : ex2((m - m_end) * c2));
     named_bar_sync(1, 256);
     const float total = s_l[0][row] + s_l[1][row];
+    // (not earlier: join_kernel's CTAs would crowd onto the few SMs that have no CTA of this kernel)
+    pdl_trigger();
     // ---- epilogue: O / l, half the dims each
     const bool zero = p < 0, lost = tile.over || !ok;
     const int d0 = grp * (D / 2);
@@ -766,16 +772,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(
       const Parts parts = parts_of(ws, int64_t(gridDim.x) * gridDim.y, D);
       if (row_live && grp == 0)
         parts.ml[part * kRows + row] = make_float2(m_end == -INFINITY ? -INFINITY : m_end * c2, lost ? NAN : total);
-      float* out = parts.o + (part * kRows + row) * D;
+      float4* out = part_row<D>(parts, part, row);
 #pragma unroll 1
-      for (int d = d0; d < d0 + D / 2 && n_tiles > 0; d += 16) {
-        uint32_t r[16];
-        tmem_ld16(tm_o + tl + d, r);
+      for (int d = d0; d < d0 + D / 2 && n_tiles > 0; d += 32) {
+        uint32_t r[32];
+        tmem_ld32(tm_o + tl + d, r);
         tmem_ld_wait();
         if (row_live)
 #pragma unroll
-          for (int e = 0; e < 16; e += 4)
-            *reinterpret_cast<uint4*>(out + d + e) = uint4{r[e], r[e + 1], r[e + 2], r[e + 3]};
+          for (int e = 0; e < 32; e += 4)
+            *reinterpret_cast<uint4*>(out + (d + e) / 4 * kRows) = uint4{r[e], r[e + 1], r[e + 2], r[e + 3]};
       }
     } else {
       __nv_bfloat16* out = a.out + (int64_t(tile.t0 + tok) * a.Hq + int64_t(h) * G + g) * D + d0;
@@ -815,38 +821,59 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(
   }
 }
 
-// Joins the parts of a split call: a warp per row of a block, D/32 dims a lane.
+// Joins the parts of a split call: a thread has 16 dims of a row, so that a warp's loads lie side
+// by side in the parts and each thread writes a whole 32-byte sector.
 template <int D>
-__global__ void __launch_bounds__(256) join_kernel(const AttnArgs a, void* ws, int splits) {
-  const int G = a.Hq / a.kv.Hkv, per = kRows / G, lane = threadIdx.x & 31;
+__global__ void __launch_bounds__(2 * kRows) join_kernel(const AttnArgs a, void* ws, int splits) {
+  const int G = a.Hq / a.kv.Hkv, per = kRows / G, row = threadIdx.x % kRows;
+  const int d0 = blockIdx.y * 32 + threadIdx.x / kRows * 16;
   const int block = blockIdx.x, h = block % a.kv.Hkv;
   const int x = int(gridDim.x) / a.kv.Hkv - 1 - block / a.kv.Hkv;
   TileOf tile;
+  // (the lengths are older than the main kernel, which has waited for whatever wrote them)
   const bool any = find_tile(a, per, x, &tile);
   pdl_wait();
-  if (!any) return;
+  if (!any || row >= tile.n * G) return;
   const Parts parts = parts_of(ws, int64_t(gridDim.x) * splits, D);
-  for (int row = blockIdx.y * 8 + (threadIdx.x >> 5); row < tile.n * G; row += gridDim.y * 8) {
-    const int tok = row / G, p = tile.p0 + tok;
-    const int64_t at = (int64_t(block) * splits * kRows + row);
-    float top = -INFINITY;
-    for (int s = 0; s < splits; ++s) top = fmaxf(top, parts.ml[at + int64_t(s) * kRows].x);
-    const float base = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, acc[D / 32] = {};
-    for (int s = 0; s < splits; ++s) {
-      const float2 ml = parts.ml[at + int64_t(s) * kRows];
-      if (ml.x == -INFINITY && ml.y == 0.f) continue;  // no key there: its O may be unwritten
-      const float f = ex2(ml.x - base);
-      sum += ml.y * (ml.x == -INFINITY ? 1.f : f);
+  const float2* ml = parts.ml + int64_t(block) * splits * kRows + row;
+  const float4* o = part_row<D>(parts, int64_t(block) * splits, row) + d0 / 4 * kRows;
+  float top = -INFINITY;
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s) top = fmaxf(top, ml[s * kRows].x);
+  const float base = top == -INFINITY ? 0.f : top;
+  float sum = 0.f;
+  float4 acc[4] = {};
+#pragma unroll 2
+  for (int s = 0; s < splits; ++s, o += kRows * D / 4) {
+    const float2 m = ml[s * kRows];
+    if (m.x == -INFINITY && m.y == 0.f) continue;  // no key there: its O may be unwritten
+    const float f = ex2(m.x - base);
+    sum += m.y * (m.x == -INFINITY ? 1.f : f);
 #pragma unroll
-      for (int e = 0; e < D / 32; ++e)
-        acc[e] += f * parts.o[(at + int64_t(s) * kRows) * D + lane + 32 * e];
+    for (int e = 0; e < 4; ++e) {
+      const float4 y = o[e * kRows];
+      acc[e].x += f * y.x;
+      acc[e].y += f * y.y;
+      acc[e].z += f * y.z;
+      acc[e].w += f * y.w;
     }
-    __nv_bfloat16* out = a.out + (int64_t(tile.t0 + tok) * a.Hq + int64_t(h) * G + row % G) * D;
-#pragma unroll
-    for (int e = 0; e < D / 32; ++e)
-      out[lane + 32 * e] = __float2bfloat16_rn(tile.over ? NAN : p < 0 ? 0.f : acc[e] / sum);
   }
+  const int tok = row / G;
+  const bool zero = tile.p0 + tok < 0;
+  const float inv = 1.f / sum;
+  uint32_t y[8];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float4 v = acc[e];
+    y[2 * e] = pack_bf16(zero ? 0.f : v.x * inv, zero ? 0.f : v.y * inv);
+    y[2 * e + 1] = pack_bf16(zero ? 0.f : v.z * inv, zero ? 0.f : v.w * inv);
+  }
+  if (tile.over)
+    for (int e = 0; e < 8; ++e) y[e] = pack_bf16(NAN, NAN);
+  uint4* out = reinterpret_cast<uint4*>(
+      a.out + (int64_t(tile.t0 + tok) * a.Hq + int64_t(h) * G + row % G) * D + d0);
+  out[0] = uint4{y[0], y[1], y[2], y[3]};
+  out[1] = uint4{y[4], y[5], y[6], y[7]};
 }
 
 bool page_map(CUtensorMap* map, const PagedKV& kv, const __nv_bfloat16* base, int64_t page_stride,
@@ -864,16 +891,30 @@ struct Plan {
   int splits;
   int64_t slots;  // of find_tile
 };
+// Slots that find_tile uses: floor(cu / per) + ceil(n / per) <= ceil((cu + n) / per).
+int64_t slots_of(int T, int B, int per) { return (int64_t(T) + per - 1) / per + B - 1; }
+// `keys`: the most that a row may see.
+//
+// Split: while the parts still fit on the GPU at once (152 CTAs took 69 us where 114 took 49), and
+// no further than a part's tiles and the join cost the same: a tile takes about 1.2 us, joining
+// one more part 0.4, so sqrt(3 tiles) parts.  64 tokens on 8000 keys, 2 heads of 256: 100 us whole,
+// 26.5 in 13 to 16 parts, 39 in 24; one token on 30000 keys: 338 whole, 37 in 24 parts, 50 in
+// 74.  Below 6 tiles the join costs what it saves (16 x 8 tokens on 600 keys: 17.8 whole, 18.4 in
+// 2; 4 heads of 128: 13.9 and 16.8).
+//
+// Pairs: at D = 256, where sequences have two CTAs' rows: one prompt of 8192 tokens 400 us, 476
+// in single CTAs; 16 tokens each for 64 sequences 107 and 79.  At D = 128 a lone CTA hides its
+// copies: 2 x 4096 tokens 32/4 heads of 128 took 1 to 8 % longer in pairs.
 Plan plan_of(int T, int B, int Hq, int Hkv, int D, int64_t keys) {
   const int per = kRows / (Hq / Hkv);
-  const int64_t slots = int64_t(T) / per + B;
-  const int64_t tiles = int64_t(T) / per > B ? int64_t(T) / per : B;  // about what is there
-  // few rows: enough CTAs for the GPU, two tiles of keys each at least
-  int64_t splits = 148 / (tiles * Hkv);
-  if (splits > keys / (2 * kTile)) splits = keys / (2 * kTile);
-  if (splits > 1) return {false, int(splits), slots};
-  const bool pair = D >= 128 && int64_t(T) / per >= 2 * int64_t(B);
-  return {pair, 1, pair ? int64_t(T) / (2 * per) + B : slots};
+  const int64_t slots = slots_of(T, B, per), rows = (int64_t(T) + per - 1) / per;
+  const int64_t tiles = (keys + kTile - 1) / kTile;
+  const int64_t most = 148 / (std::max<int64_t>(rows, B) * Hkv);
+  int splits = 1;
+  while (tiles >= 6 && splits < most && int64_t(splits + 1) * (splits + 1) <= 3 * tiles) ++splits;
+  if (splits > 1) return {false, splits, slots};
+  const bool pair = D == 256 && rows >= 2 * int64_t(B);
+  return {pair, 1, pair ? slots_of(T, B, 2 * per) : slots};
 }
 
 template <int D, bool PAIR>
@@ -895,7 +936,8 @@ cudaError_t launch_one(const AttnArgs& a, const Plan& plan, void* ws, cudaStream
                                    dim3(unsigned(blocks * C::kN), unsigned(plan.splits)), kThreads,
                                    C::kSmem, C::kN, st, mq, mk, mv, a, ws);
   if (e != cudaSuccess || plan.splits == 1) return e;
-  return launch_dependent(join_kernel<D>, dim3(unsigned(blocks), 4), 256, 0, 1, st, a, ws, plan.splits);
+  return launch_dependent(join_kernel<D>, dim3(unsigned(blocks), D / 32), 2 * kRows, 0, 1, st, a, ws,
+                          plan.splits);
 }
 
 template <int D, bool PAIR> cudaError_t init_one() {
@@ -908,8 +950,7 @@ template <int D, bool PAIR> cudaError_t init_one() {
 cudaError_t attn_prefill_init() {
   cudaError_t e;
   if ((e = init_one<64, false>()) != cudaSuccess || (e = init_one<128, false>()) != cudaSuccess ||
-      (e = init_one<256, false>()) != cudaSuccess || (e = init_one<128, true>()) != cudaSuccess ||
-      (e = init_one<256, true>()) != cudaSuccess)
+      (e = init_one<256, false>()) != cudaSuccess || (e = init_one<256, true>()) != cudaSuccess)
     return e;
   return cudaSuccess;
 }
@@ -922,12 +963,14 @@ size_t attn_prefill_ws_bytes(int T, int B, int Hq, int Hkv, int D, int64_t keys)
 cudaError_t launch_attn_prefill(const AttnArgs& args, void* ws, cudaStream_t st) {
   AttnArgs a = args;
   if (a.T == 0) return cudaSuccess;
-  const Plan p = plan_of(a.T, a.kv.B, a.Hq, a.kv.Hkv, a.kv.D,
-                         int64_t(a.kv.max_pages) << a.kv.page_shift);
+  int64_t keys = int64_t(a.kv.max_pages) << a.kv.page_shift;
+  if (a.window > 0)  // (a window's tiles may begin and end inside, the sinks' end inside)
+    keys = std::min(keys, int64_t(a.window) + a.sinks + 3 * kTile);
+  const Plan p = plan_of(a.T, a.kv.B, a.Hq, a.kv.Hkv, a.kv.D, keys);
   if (a.kv.n_pages == 0) a.kv.max_pages = 0;  // no page: every row with keys gets NaN
   switch (a.kv.D) {
     case 64: return launch_one<64, false>(a, p, ws, st);
-    case 128: return p.pair ? launch_one<128, true>(a, p, ws, st) : launch_one<128, false>(a, p, ws, st);
+    case 128: return launch_one<128, false>(a, p, ws, st);
     default: return p.pair ? launch_one<256, true>(a, p, ws, st) : launch_one<256, false>(a, p, ws, st);
   }
 }

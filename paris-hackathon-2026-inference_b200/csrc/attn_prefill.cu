@@ -20,14 +20,16 @@
 //
 // Warps 0-7: softmax and epilogue; warps 8 and 9: TMA of K (and Q) and of V, each through a ring
 // of 16 KiB chunks; warps 10 and 11: the products S and P V (a pair's first CTA issues for
-// both, and both CTAs' copies report to its barriers).
+// both, and both CTAs' copies report to its barriers); warps 12-15 clean V where rows do not
+// see all of it.
 //
 // Few rows: the keys are split over several CTAs (gridDim.y), whose parts join_kernel joins.
 //
 // Values that a row does not see must not reach its sum even where they are not finite, but
-// 0 x inf is NaN: in tiles at an edge of some row's sight, V rows that nobody sees or that
+// 0 x inf is NaN: in tiles that are cut by some row's sight, V rows that nobody sees or that
 // hold a non-finite number are zeroed in shared memory, and the latter are added to the rows
-// that see them one by one.
+// that see them one by one.  Warps of their own look at the tile as it lands (in the softmax
+// warps, from global memory, that cost 260 us instead of 2 for XXX).
 #include <algorithm>
 
 #include "paged.cuh"
@@ -37,8 +39,13 @@ namespace pmoe {
 
 namespace {
 
-constexpr int kRows = 128, kTile = 128, kThreads = 384, kChunk = 16384;
+constexpr int kRows = 128, kTile = 128, kThreads = 512, kChunk = 16384;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kCuts = 8;      // tiles with keys that some rows do not see, at a time
+// Registers of a thread: the launch's, which init_one checks, dealt out to the roles (a sum above
+// the launch's would wait for ever).  The softmax warps hold a row of S.
+constexpr int kRegs = 128, kRegsSoftmax = 200, kRegsIssue = 64, kRegsClean = 48;
+static_assert(256 * kRegsSoftmax + 128 * kRegsIssue + 128 * kRegsClean <= kThreads * kRegs, "");
 constexpr float kGrow = 8.f;  // powers of two that a row's maximum may lag behind
 
 template <int D, bool PAIR> struct Cfg {
@@ -208,6 +215,16 @@ template <bool PAIR> __device__ __forceinline__ void tmem_signal(uint64_t* bar) 
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity));
 }
+__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_n(uint64_t* bar, uint32_t n) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(n) : "memory");
+}
+__device__ __forceinline__ void st_cluster(uint32_t cluster_addr, uint32_t x) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(x) : "memory");
+}
 // The n lowest bits (n <= 0: none, n >= 32: all).
 __device__ __forceinline__ uint32_t low_bits(int n) {
   return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1;
@@ -276,15 +293,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(
   char* s_q = smem;                    // [D/64][128 rows][128 bytes], swizzled
   char* s_k = smem + kRows * D * 2;    // the rings
   char* s_v = s_k + C::kSlots * kChunk;
-  // full: a chunk has landed, in both CTAs (the first CTA's barrier counts); local: this CTA's
-  // part of a V chunk that its softmax warps clean first (other chunks pass it at once)
-  __shared__ uint64_t k_full[C::kSlots], k_empty[C::kSlots];
-  __shared__ uint64_t v_full[C::kSlots], v_empty[C::kSlots], v_local[C::kSlots];
+  // full: a chunk has landed, in both CTAs (the first CTA's barrier counts), and is clean.
+  // Tiles that are cut (cut_of): cut_full: of their u-th chunk of V at u % 8: this CTA's part has
+  // landed; p_cut: of the e-th tile at e % 8: its weights are written; bad_known at e % 2: s_bad is
+  // there, from both CTAs.  (The rings hold 6 chunks at most, so that chunk u + 8 is fetched, and
+  // tile e + 8 met, after tile e's product, which waits for all who use these.)
+  __shared__ uint64_t k_full[C::kSlots], k_empty[C::kSlots], v_full[C::kSlots], v_empty[C::kSlots];
+  __shared__ uint64_t cut_full[kCuts], p_cut[kCuts], bad_known[2];
   __shared__ uint64_t s_full[2], s_free[C::kS], p_ready[2][2], pv_done[2], q_full;
   __shared__ uint32_t s_tmem;
   __shared__ int s_first;              // tile 0 adds to O (set to zero before) instead of setting it
-  __shared__ uint16_t s_bad[2][8];     // per group: keys of the tile whose V row is not finite
-  __shared__ float s_m[kRows], s_l[2][kRows];
+  __shared__ uint32_t s_bad[2][D / 64][4];  // keys of a cut tile whose V, in those 64 dims, is not
+                                            // finite and not seen by all rows
+  __shared__ float s_m[kRows];
 
   // (shuffled, so that the compiler sees one value per warp and keeps the roles' addresses
   // in uniform registers)
@@ -322,10 +343,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(
     return (j < ns ? j : w0 + j - ns) * kTile;
   };
 
-  // a missing page where some row looks: every tile is an edge (found below)
-  auto edge_of = [&](int j, bool hole) {  // may some row not see some key of the tile?
+  auto cut_of = [&](int j) {  // may some row not see some key of the tile?
     const int k0 = tile_key(j);
-    return hole || tile.p0 < 0 || k0 + kTile - 1 > tile.p0 || (k0 < lo_max && k0 + kTile > sink_all);
+    return tile.p0 < 0 || k0 + kTile - 1 > tile.p0 || (k0 < lo_max && k0 + kTile > sink_all);
   };
 
   if (warp == 10) {
@@ -341,10 +361,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(
     for (int i = 0; i < C::kSlots; ++i) {
       mbar_init(&k_full[i], 1);
       mbar_init(&k_empty[i], 1);
-      mbar_init(&v_full[i], 1);
+      mbar_init(&v_full[i], 4 * C::kN);
       mbar_init(&v_empty[i], 1);
-      mbar_init(&v_local[i], 1);
     }
+    for (int i = 0; i < kCuts; ++i) {
+      mbar_init(&cut_full[i], 1);
+      mbar_init(&p_cut[i], 4);
+    }
+    for (int i = 0; i < 2; ++i) mbar_init(&bad_known[i], 4 * C::kN);
     for (int i = 0; i < C::kS; ++i) mbar_init(&s_free[i], 4 * C::kN);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
@@ -364,9 +388,123 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(
   tc_fence_after();
   const uint32_t tm_o = __shfl_sync(0xffffffffu, s_tmem, 0), tm_p = tm_o + D, tm_s = tm_p + 128;
 
-  // (384 threads start with 168 registers each; the softmax warps hold a row of S.)
-  if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+  if (warp >= 12) {
+    // ---- V of the cut tiles: a thread has 64 dims of a key of each chunk
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsClean));
+    const int line = tid & 127, row = line % C::kVr, wc = warp & 3;
+    const int of = rank * C::kVg + wc * 32 / C::kVr;  // 64 dims of D
+    bool ok = true;
+    for (int j = 0, e = 0; j < n_tiles; ++j) {
+      if (!cut_of(j)) continue;
+      const int k0 = tile_key(j);
+      uint32_t(*bad_at)[4] = s_bad[e & 1];
+      bool any = false;
+      for (int c = 0; c < C::kVc; ++c) {
+        const int u = e * C::kVc + c;
+        // (one warp polls: four took issue slots from the softmax warps)
+        if (wc == 0) ok = warp_wait(&cut_full[u % kCuts], (u / kCuts) & 1);
+        ok = !bar_any(6, 128, !ok);
+        if (!ok) break;
+        const int jj = k0 + c * C::kVr + row;
+        const bool some = jj <= p_last && (jj < sink_any || jj >= lo_any);
+        const bool all = jj <= tile.p0 && (jj >= lo_max || jj < sink_all);
+        uint4* v = reinterpret_cast<uint4*>(s_v + (j * C::kVc + c) % C::kSlots * kChunk + line * 128);
+        bool bad = false;
+        if (some && !all) {  // (lines begin in the same bank)
+#pragma unroll 4
+          for (int i = 0; i < 8; ++i) {
+            const uint4 x = v[(i + lane) & 7];
+            bad |= nonfinite2(x.x) || nonfinite2(x.y) || nonfinite2(x.z) || nonfinite2(x.w);
+          }
+        }
+        if (!some || bad)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[(i + lane) & 7] = uint4{0, 0, 0, 0};
+        const uint32_t who = __ballot_sync(0xffffffffu, bad);
+        if (lane == 0) {
+          uint32_t* word = &bad_at[of][(c * C::kVr + wc * 32 % C::kVr) / 32];
+          if (PAIR) {
+            st_cluster(mapa_shared(smem_u32(word), 0), who);
+            st_cluster(mapa_shared(smem_u32(word), 1), who);
+          } else {
+            *word = who;
+          }
+        }
+        any |= who != 0;
+      }
+      if (!ok) break;
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (PAIR) {  // what either CTA found: the product adds both halves of the dims to both's rows
+        if (lane == 0)
+          for (int cta = 0; cta < 2; ++cta) mbar_arrive_cluster(mapa_shared(smem_u32(&bad_known[e & 1]), cta));
+        ok = __all_sync(0xffffffffu, mbar_wait_cluster(&bad_known[e & 1], (e >> 1) & 1));
+        for (int w = 0; w < D / 16; ++w) any |= *(volatile uint32_t*)&bad_at[w / 4][w % 4] != 0;
+      } else {
+        any = bar_any(6, 128, any);
+      }
+      if (ok && any) {
+        // What was taken out because not all rows see it and it is not finite: added to the
+        // rows that do (thread = row from here), between the products of tiles j - 1 and j.
+        ok = warp_wait(&p_cut[e % kCuts], (e / kCuts) & 1);
+        // (the barrier's use before, tile j - 3, has ended: the weights were written after j - 2's)
+        if (j > 0) ok = ok && warp_wait(&pv_done[(j - 1) & 1], ((j - 1) >> 1) & 1);
+        tc_fence_after();
+        const uint32_t tl = uint32_t(wc) << 21, o = tm_o + tl, tp = tm_p + tl + (j & 1) * 64;
+        const int tok = rank * per + line / G;
+        const int p = line / G < per && tok < tile.n ? tile.p0 + tok : -1;
+        int lo = 0, sink = 0;
+        if (p >= 0) visible_keys(p, a.window, a.sinks, &lo, &sink);
+        if (j == 0) {
+          const uint32_t zero[16] = {};
+          for (int d = 0; d < D; d += 16) tmem_st16(o + d, zero);
+          tmem_st_wait();
+          if (line == 0) *(volatile int*)&s_first = 1;
+        }
+        for (int w = 0; w < 4 && ok; ++w) {
+          uint32_t left = 0;
+          for (int x = 0; x < D / 64; ++x) left |= bad_at[x][w];
+          while (left) {
+            const int bit = __ffs(left) - 1, key = w * 32 + bit, jk = k0 + key;
+            left &= left - 1;
+            const uint32_t pw = tmem_ld1(tp + key / 2);
+            tmem_ld_wait();
+            const float pk = __uint_as_float(key & 1 ? pw & 0xffff0000u : pw << 16);
+            const int page = page_of(a.kv, tile.b, jk);
+            const bool mine = page >= 0 && jk <= p && (jk < sink || jk >= lo);
+            const __nv_bfloat16* vr = a.kv.v + max(page, 0) * a.kv.v_page_stride +
+                                      ((int64_t(h) << a.kv.page_shift) + (jk & ((1 << a.kv.page_shift) - 1))) * D;
+            for (int d = 0; d < D; d += 16) {
+              if (!(bad_at[d / 64][w] >> bit & 1)) continue;  // left in the product
+              uint32_t x[16];
+              tmem_ld16(o + d, x);
+              tmem_ld_wait();
+              if (mine)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                  x[i] = __float_as_uint(fmaf(pk, __bfloat162float(vr[d + i]), __uint_as_float(x[i])));
+              tmem_st16(o + d, x);
+            }
+            tmem_st_wait();
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+      }
+      if (!ok) break;
+      if (lane == 0)
+        for (int c = 0; c < C::kVc; ++c) {
+          uint64_t* bar = &v_full[(j * C::kVc + c) % C::kSlots];
+          if (PAIR)
+            mbar_arrive_cluster(mapa_shared(smem_u32(bar), 0));
+          else
+            mbar_arrive(bar);
+        }
+      __syncwarp();
+      ++e;
+    }
+  } else if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
     if (warp < 10) {
       // ---- TMA of one operand
       const bool is_v = warp == 9;
@@ -390,30 +528,24 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(
       auto pages_of = [&](int j) {  // lane i: the tile's i-th page
         return j < n_tiles && lane < per_tile ? page_of(a.kv, tile.b, tile_key(j) + lane * ps) : -1;
       };
-      int next = pages_of(0), slot = 0, use = 0;
-      bool hole = false;
-      if (is_v && n_tiles > 0) {
-        for (int i = lane; i < (sink_any + ps - 1) >> sh; i += 32) hole |= page_of(a.kv, tile.b, i << sh) < 0;
-        for (int i = (lo_any >> sh) + lane; i <= p_last >> sh; i += 32)
-          hole |= page_of(a.kv, tile.b, i << sh) < 0;
-        hole = __any_sync(0xffffffffu, hole);
-      }
+      int next = pages_of(0), slot = 0, use = 0, cuts = 0;
       bool ok = true;
       int seq = 0;
       for (int j = 0; j < n_tiles && ok; ++j) {
         const int page = next;
         next = pages_of(j + 1);
-        const bool clean = is_v && edge_of(j, hole);
+        const bool cut = is_v && cut_of(j);
         for (int c = 0; c < C::kKc; ++c, ++seq) {
           if (use > 0) ok = warp_wait(&empty[slot], (use - 1) & 1);
           if (!ok) break;
+          uint64_t* landed = &cut_full[cuts % kCuts];
+          cuts += cut;
           if (lane == 0) {
-            if (clean) {
-              if (rank == 0) mbar_arrive(&full[slot]);
-              mbar_arrive_expect_tx(&v_local[slot], kChunk);
-            } else {
-              if (rank == 0) mbar_arrive_expect_tx(&full[slot], C::kN * kChunk);
-              if (is_v) mbar_arrive(&v_local[slot]);
+            if (cut) {
+              mbar_arrive_expect_tx(landed, kChunk);
+            } else if (rank == 0) {
+              mbar_expect_tx(&full[slot], C::kN * kChunk);
+              mbar_arrive_n(&full[slot], is_v ? 4 * C::kN : 1);
             }
           }
           __syncwarp();
@@ -423,16 +555,17 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(
           if (r < keys)
             tma_box<PAIR>(ring + slot * kChunk + (grp * keys + r) * 128, is_v ? &map_v : &map_k,
                           key & (ps - 1), cg, h, at < 0 ? a.kv.n_pages : at,  // no page: zeros
-                          clean ? smem_u32(&v_local[slot]) : first_full + slot * 8);
+                          cut ? smem_u32(landed) : first_full + slot * 8);
           slot = slot + 1 == C::kSlots ? 0 : slot + 1;
           use += slot == 0;
         }
       }
-      if (!ok)  // a wait ran out: let the copies land before the CTA ends
-        for (int q = max(0, seq - C::kSlots); q < seq; ++q) {
-          if (rank == 0) mbar_wait(&full[q % C::kSlots], (q / C::kSlots) & 1);
-          if (is_v) mbar_wait(&v_local[q % C::kSlots], (q / C::kSlots) & 1);
-        }
+      if (!ok) {  // a wait ran out: let the copies land before the CTA ends
+        for (int q = max(0, seq - C::kSlots); q < seq; ++q)
+          if (rank == 0 && !(is_v && cut_of(q / C::kVc)))
+            mbar_wait(&full[q % C::kSlots], (q / C::kSlots) & 1);
+        for (int u = max(0, cuts - C::kSlots); u < cuts; ++u) mbar_wait(&cut_full[u % kCuts], (u / kCuts) & 1);
+      }
     } else {
       // ---- the products: a warp each for S and P V walks and waits, one lane issues.  (A warp
       // of its own for each: one warp for both spent 3300 cycles a tile on waits and issue, the
@@ -517,7 +650,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(
     }
   } else {
     // ---- softmax: group = warps 0-3 or 4-7, thread = row
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
     const int grp = warp >> 2, wq = warp & 3, row = tid & 127;
     const uint32_t tl = uint32_t(wq) << 21;  // this warp's TMEM lanes
     const int tok = rank * per + row / G, g = row % G;
@@ -549,44 +682,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(
     };
     // A wait that runs out makes the warp's rows NaN; it goes on through the tiles without
     // waiting, as the others may stand at the groups' barriers.
+    int cuts = 0;
     for (int j = grp; j < n_tiles; j += 2) {
       const int k0 = tile_key(j);
       const int buf = j % C::kS;
       const uint32_t ts = tm_s + tl + buf * kTile, tp = tm_p + tl + grp * 64;
-      const bool edge = edge_of(j, hole);
-      uint32_t bad = 0;  // of this warp's 32 keys
-      if (edge) {
-        // V rows of this tile that some rows see and others do not, and that are not finite; a
-        // warp has 32 keys, D/8 lanes a row.  (From global memory: a pair's CTAs hold half the
-        // dims each.  All loads at once: one latency.)
-        constexpr int kLanes = D / 8, kAt = 32 / kLanes;
-        const int j0 = k0 + wq * 32;  // two runs of 16 keys, each within a page
-        const int pages[2] = {page_of(a.kv, tile.b, j0), page_of(a.kv, tile.b, j0 + 16)};
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const __nv_bfloat16* v0 = a.kv.v + max(pages[half], 0) * a.kv.v_page_stride +
-                                    ((int64_t(h) << a.kv.page_shift) + ((j0 + 16 * half) & ((1 << a.kv.page_shift) - 1))) * D +
-                                    8 * (lane % kLanes);
-          uint4 v[16 / kAt];
-#pragma unroll
-          for (int i = 0; i < 16 / kAt; ++i) {
-            const int key = i * kAt + lane / kLanes, jj = j0 + 16 * half + key;
-            const bool some = jj <= p_last && (jj < sink_any || jj >= lo_any);
-            const bool all = jj <= tile.p0 && (jj >= lo_max || jj < sink_all);
-            v[i] = uint4{0, 0, 0, 0};
-            if (pages[half] >= 0 && some && !all) v[i] = *reinterpret_cast<const uint4*>(v0 + key * D);
-          }
-#pragma unroll
-          for (int i = 0; i < 16 / kAt; ++i) {
-            const uint32_t who = __ballot_sync(
-                0xffffffffu, nonfinite2(v[i].x) || nonfinite2(v[i].y) || nonfinite2(v[i].z) || nonfinite2(v[i].w));
-#pragma unroll
-            for (int k = 0; k < kAt; ++k)
-              if (who >> (k * kLanes) & (kLanes == 32 ? 0xffffffffu : (1u << kLanes % 32) - 1))
-                bad |= 1u << (16 * half + i * kAt + k);
-          }
-        }
-      }
+      cuts += j > 0 && cut_of(j - 1);
+      const int e_cut = cuts;
+      const bool cut = cut_of(j);
+      cuts += cut;
       ok = ok && warp_wait(&s_full[grp], (j >> 1) & 1);
       tc_fence_after();
       uint32_t r[4][32];
@@ -596,7 +700,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(
       tc_fence_before();
       __syncwarp();
       if (lane == 0) tmem_signal<PAIR>(&s_free[buf]);
-      if (edge) {
+      if (cut || hole) {
         // What the row does not see at -inf, as bits of the tile's keys: 0..hi but not
         // [a, b).  (A comparison per element took 7000 cycles a tile, most of it fetching code.)
         const int hi = p - k0, ka = sink - k0, kb = lo - k0;
@@ -677,7 +781,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(
         }
         if (c == 0 && j >= 2) wait_pv(j - 2);  // this group's P buffer is free
         tmem_st16(tp + c * 16, w);
-        if (c == 1 && !edge) {
+        if (c == 1) {
           tmem_st_wait();
           tc_fence_before();
           __syncwarp();
@@ -686,82 +790,22 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(
       }
       l += sum.x + sum.y;
       tmem_st_wait();
-      if (edge) {
-        // Clean V of this tile: thread = key.  The slots' uses before this one have to have landed
-        // for the barriers' parity to be this use's: they belong to tile j - 2 or before, whose
-        // product has ended, or, in a short ring, to tile j - 1.
-        if (C::kSlots < 2 * C::kVc && j > 0) wait_pv(j - 1);
-        const int vseq = j * C::kVc, q = vseq + row / C::kVr;
-        for (int c = 0; c < C::kVc; ++c)
-          ok = ok && warp_wait(&v_local[(vseq + c) % C::kSlots], ((vseq + c) / C::kSlots) & 1);
-        char* vrow = s_v + (q % C::kSlots) * kChunk + (row % C::kVr) * 128;
-        const int jj = k0 + row;
-        const bool seen = jj <= p_last && (jj < sink_any || jj >= lo_any);
-        if (ok && (!seen || (bad >> lane & 1)))
-          for (int i = 0; i < C::kVg * 8; ++i)
-            *reinterpret_cast<uint4*>(vrow + (i >> 3) * C::kVr * 128 + (((i + lane) & 7) << 4)) = uint4{0, 0, 0, 0};
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        if (lane == 0) {
-          s_bad[grp][2 * wq] = uint16_t(bad);
-          s_bad[grp][2 * wq + 1] = uint16_t(bad >> 16);
-        }
-        if (bar_any(4 + grp, 128, bad != 0)) {
-          // add these keys to the rows that see them, before the tile's product
-          if (j > 0) wait_pv(j - 1);
-          if (j == 0) {
-            const uint32_t zero[16] = {};
-            for (int d = 0; d < D; d += 16) tmem_st16(tm_o + tl + d, zero);
-            tmem_st_wait();
-            if (row == 0) *(volatile int*)&s_first = 1;
-          }
-          for (int w = 0; w < 8 && ok; ++w) {
-            uint32_t left = s_bad[grp][w];
-            while (left) {
-              const int key = w * 16 + __ffs(left) - 1;
-              left &= left - 1;
-              const uint32_t pw = tmem_ld1(tp + key / 2);
-              tmem_ld_wait();
-              const float pk = __uint_as_float(key & 1 ? pw & 0xffff0000u : pw << 16);
-              const int jk = k0 + key;
-              const bool mine = jk <= p && (jk < sink || jk >= lo);
-              const int page = page_of(a.kv, tile.b, jk);
-              const __nv_bfloat16* vr = a.kv.v + max(page, 0) * a.kv.v_page_stride +
-                                        ((int64_t(h) << a.kv.page_shift) + (jk & ((1 << a.kv.page_shift) - 1))) * D;
-              for (int d = 0; d < D; d += 16) {
-                uint32_t r[16];
-                tmem_ld16(tm_o + tl + d, r);
-                tmem_ld_wait();
-                if (mine && page >= 0)
-#pragma unroll
-                  for (int e = 0; e < 16; ++e)
-                    r[e] = __float_as_uint(fmaf(pk, __bfloat162float(vr[d + e]), __uint_as_float(r[e])));
-                tmem_st16(tm_o + tl + d, r);
-              }
-              tmem_st_wait();
-            }
-          }
-          bar_any(4 + grp, 128, false);  // s_bad is free again
-        }
-      }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
-        if (edge) {  // V in shared memory has been written too
-          mbar_arrive_cluster(mapa_shared(smem_u32(&p_ready[grp][0]), 0));
-          mbar_arrive_cluster(mapa_shared(smem_u32(&p_ready[grp][1]), 0));
-        } else {
-          tmem_signal<PAIR>(&p_ready[grp][1]);
-        }
+        if (cut) mbar_arrive(&p_cut[e_cut % kCuts]);
+        tmem_signal<PAIR>(&p_ready[grp][1]);
       }
     }
     if (n_tiles > 1) wait_pv(n_tiles - 2);
     if (n_tiles > 0) wait_pv(n_tiles - 1);
-    // ---- the groups' sums, each brought to the last maximum
+    // ---- the groups' sums, each brought to the last maximum (in the place of Q, which is done)
+    float* s_l = reinterpret_cast<float*>(s_q);
     named_bar_sync(1, 256);
     const float m_end = n_tiles > 0 ? s_m[row] : -INFINITY;
-    s_l[grp][row] = l * (m == m_end ? 1.f : m == -INFINITY ? 0.f : ex2((m - m_end) * c2));
+    s_l[grp * kRows + row] = !ok ? NAN : l * (m == m_end ? 1.f : m == -INFINITY ? 0.f : ex2((m - m_end) * c2));
     named_bar_sync(1, 256);
-    const float total = s_l[0][row] + s_l[1][row];
+    const float total = s_l[row] + s_l[kRows + row];
     // (not earlier: join_kernel's CTAs would crowd onto the few SMs that have no CTA of this kernel)
     pdl_trigger();
     // ---- epilogue: O / l, half the dims each
@@ -941,6 +985,11 @@ cudaError_t launch_one(const AttnArgs& a, const Plan& plan, void* ws, cudaStream
 }
 
 template <int D, bool PAIR> cudaError_t init_one() {
+  // the registers that the roles share out are those of the launch
+  cudaFuncAttributes f{};
+  const cudaError_t e = cudaFuncGetAttributes(&f, attn_prefill_kernel<D, PAIR>);
+  if (e != cudaSuccess) return e;
+  if (f.numRegs != kRegs) return cudaErrorInvalidDeviceFunction;
   return cudaFuncSetAttribute(attn_prefill_kernel<D, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                               Cfg<D, PAIR>::kSmem);
 }

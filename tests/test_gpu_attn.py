@@ -257,6 +257,31 @@ def test_prefill_nonfinite_keys_and_values_stay_behind_the_mask(D, Hq, bad):
                 assert torch.equal(torch.isnan(got) | torch.isinf(got), ~fine)
 
 
+@pytest.mark.parametrize("window,sinks", [(0, 0), (180, 70)])
+@pytest.mark.parametrize("D,Hq", [(64, 1), (64, 16), (128, 1), (128, 16), (256, 1), (256, 16)])
+def test_prefill_many_nonfinite_values_in_all_dims(D, Hq, window, sinks):
+    """Values that are not finite in every tile, at every 64 dims: each row has them in exactly
+    the dims and from the keys that it sees."""
+    from paris_moe_b200 import ops
+    new, ctx = [300, 290], [500, 0]
+    lens = [a + b for a, b in zip(new, ctx)]
+    pages, table, n = make_cache(lens, 1, D, 32, layers=1)
+    g = torch.Generator().manual_seed(D + Hq + window)
+    for b in (0, 1):
+        for j in torch.randperm(lens[b], generator=g)[:40].tolist():
+            d = int(torch.randint(0, D, (1,), generator=g))
+            bad = (math.nan, math.inf, -math.inf)[j % 3]
+            pages[table[b, j // 32].item(), 0, 1, 0, j % 32, d] = bad
+    q, cu = rand_q(sum(new), Hq, D), cu_of(new)
+    args = (table, n, cu, 0.02, window, sinks)
+    got = ops.attn_prefill(q, pages[:, 0, 0], pages[:, 0, 1], *args).cpu()
+    want, bound = R.attention(q, pages[:, 0, 0], pages[:, 0, 1], *args)
+    fine = torch.isfinite(want)
+    assert 0 < int(fine.sum()) < fine.numel()
+    assert torch.equal(torch.isfinite(got), fine)
+    assert float(((got.double() - want).abs() / bound)[fine].max()) <= 1.0
+
+
 def test_prefill_of_single_tokens_agrees_with_decode():
     from paris_moe_b200 import ops
     lens = [1, 64, 100, 333]

@@ -255,10 +255,14 @@ int to_int(const char* op, const char* name, int64_t v) {
 // Element stride of a dimension; one of at most one entry is never stepped over.
 int64_t stride_of(const Tensor& t, int dim) { return t.size(dim) <= 1 ? 0 : t.stride(dim); }
 
-// Rows [T, heads, D]: any token and head stride, contiguous heads.
-void check_rows(const char* op, const char* name, const Tensor& t, const Tensor& x) {
+void check_no_grad(const char* op, const char* name, const Tensor& t) {
   TORCH_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()), "paris_moe.", op, ": ", name,
               " requires grad, and the operator has no backward pass (call it under no_grad)");
+}
+
+// Rows [T, heads, D]: any token and head stride, contiguous heads.
+void check_rows(const char* op, const char* name, const Tensor& t, const Tensor& x) {
+  check_no_grad(op, name, t);
   TORCH_CHECK(t.is_cuda(), "paris_moe.", op, ": ", name, " must be a CUDA tensor");
   TORCH_CHECK(t.device() == x.device(), "paris_moe.", op, ": ", name, " is on ", t.device(),
               ", expected ", x.device());
@@ -278,6 +282,7 @@ CacheView check_cache(const char* op, const Tensor& q, const Tensor& k, const Te
                       const Tensor& table, const Tensor& lens) {
   for (const Tensor* t : {&k, &v}) {
     const char* name = t == &k ? "k_pages" : "v_pages";
+    check_no_grad(op, name, *t);
     TORCH_CHECK(t->is_cuda() && t->device() == q.device(), "paris_moe.", op, ": ", name,
                 " must be a CUDA tensor on ", q.device());
     TORCH_CHECK(t->scalar_type() == at::kBFloat16, "paris_moe.", op, ": ", name,
@@ -344,6 +349,7 @@ Tensor rope_append_cuda(const Tensor& q, const Tensor& k, const Tensor& v, const
               half, ", inv_freq has ", inv_freq.size(0), " entries, D/2 is ", c.D / 2);
   for (const OptTensor* w : {&w_qnorm, &w_knorm})
     if (w->has_value()) {
+      check_no_grad(op, "norm weight", **w);
       check_bf16(op, "norm weight", **w, q, 1);
       TORCH_CHECK((*w)->size(0) == c.D, "paris_moe.rope_append: norm weights must be [", c.D, "]");
     }

@@ -420,6 +420,31 @@ def test_bad_arguments_raise():
         assert torch.equal(ops.attn_decode(grad, k, v, table, n, 0.1), ops.attn_decode(q, k, v, table, n, 0.1))
 
 
+def test_caches_and_gains_that_require_grad_are_refused():
+    """They would get no gradient, so the calls raise instead."""
+    from paris_moe_b200 import ops
+    pages, table, n = make_cache([5, 9], 2, 64, 16)
+    k, v = pages[:, 0, 0], pages[:, 0, 1]
+    q, kn = rand_q(2, 4, 64), rand_q(2, 2, 64)
+    grad = pages.clone().requires_grad_()
+    for kk, vv in ((grad[:, 0, 0], v), (k, grad[:, 0, 1])):
+        with pytest.raises(RuntimeError, match="no backward pass"):
+            ops.attn_decode(q, kk, vv, table, n, 0.1)
+        with pytest.raises(RuntimeError, match="no backward pass"):
+            ops.attn_prefill(q, kk, vv, table, n, cu_of([1, 1]), 0.1)
+    at = torch.zeros(1, 2, dtype=torch.int64, device=DEV)
+    freq = torch.ones(8, device=DEV)
+    gain = torch.nn.Parameter(torch.zeros(64, dtype=torch.bfloat16, device=DEV))
+
+    def turn(wq, wk):
+        return ops.rope_append(q, kn, kn, at, freq, [8], False, k, v, table, n, w_qnorm=wq, w_knorm=wk)
+    for wq, wk in ((gain, None), (None, gain), (gain, gain)):
+        with pytest.raises(RuntimeError, match="no backward pass"):
+            turn(wq, wk)
+    with torch.no_grad():
+        assert torch.equal(turn(gain, gain), turn(gain.detach(), gain.detach()))
+
+
 # ---- rotary positions and the cache write -------------------------------------------------
 
 

@@ -28,10 +28,10 @@ __device__ __forceinline__ int rope_axis(const RopeArgs& a, int i) {
 // own = g, other = 0 behind the rotary dims.  The partner's 8 dims come from lane +- half/8 as they
 // were loaded.  A batch of rows is on its way while the angles are worked out.
 //
-// 8192 tokens of 16 + 2 heads of 256 (168 MB): 37 us, 4.5 TB/s, 70 % of the copy rate.  Bound by
+// 8192 tokens of 16 + 2 heads of 256 (168 MB): 34.5 us, 4.9 TB/s, 75 % of the copy rate.  Bound by
 // instructions (128 a row, 61 % of the issue slots): the first version took 320 a row and
 // 76 us, one with the factors in shared memory 51, this one with batches of 4 rows (110
-// registers, half the warps) 44.  64 tokens, eight warps each: 6 us, a chain of latencies.
+// registers, half the warps) 44.  64 tokens, eight warps each: 4.5 us, a chain of latencies.
 constexpr int kBatch = 2;  // row slots a warp holds at a time, and as many on their way
 
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
@@ -208,7 +208,9 @@ cudaError_t launch_split(const RopeArgs& a, cudaStream_t st) {
 
 template <int D>
 cudaError_t launch_one(const RopeArgs& a, cudaStream_t st) {
-  // warps for every SM: a warp a token for 8192 tokens, eight a token for 64
+  // Warps for every SM, and no more: a token's factors are worked out by each of its warps.  64
+  // tokens: 4.5 us with 8 warps a token, 7.5 with one; 592: 7.0 with 2, 7.2 with 8; 1024: 8.2 with
+  // 2, 11.6 with 8; 2368: 11.0 with one, 13.0 with 2.
   if (a.T >= 148 * 16) return launch_split<D, 1>(a, st);
   return a.T >= 148 * 4 ? launch_split<D, 2>(a, st) : launch_split<D, 8>(a, st);
 }

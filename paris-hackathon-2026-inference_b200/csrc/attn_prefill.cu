@@ -32,8 +32,8 @@
 // cost 2 x 4096 tokens of 32/4 heads of 128 260 us instead of 224 (215 with no cleaning at all).
 //
 // Bound by the tensor cores for long prompts at D = 256: 8192 tokens of 16/2 heads 390 us (550
-// GFLOP, 1.41 PFLOP/s, 82 % of a matrix product's best; under the power cap of a long run 447), a tile of
-// a pair 2100 cycles where the products alone need 2048.  At D = 128 and 64 by a row's softmax:
+// GFLOP, 1.41 PFLOP/s, 82 % of a matrix product's best; under the power cap of a long run 447), a
+// tile of a pair 2100 cycles where the products alone need 2048.  At D = 128 and 64 by a row's softmax:
 // 2000 cycles a tile and group, 1024 of them the exponential unit (224 us for the 2 x 4096 above,
 // 0.85 PFLOP/s).  Short calls by a block's fixed 7.5 us: 3.5 until the first S, 2.7 from the last
 // product to the end, 1.2 between blocks.

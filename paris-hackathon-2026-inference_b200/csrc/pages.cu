@@ -4,8 +4,8 @@
 // first, so the same calls give the same pages on every run.
 //
 // What a call grants depends on what the entries before it took, so one CTA plans (1024 threads,
-// marks and sums in shared memory, four refs a thread at a time): a chain of latencies, 7 to 8 us from cold caches,
-// that neither bytes nor arithmetic bound.  The copies run on the whole GPU behind it and are
+// marks and sums in shared memory, four refs a thread at a time): a chain of latencies, 7 to 8 us
+// from cold caches, that neither bytes nor arithmetic bound.  The copies run on the whole GPU behind it and are
 // bound by HBM: 32 prompts of up to 2000 tokens forked into 8 branches each, freed and grown
 // (74 MB) 24 us with the host's part, 11.4 at the copy rate; packing a pool of ten layers (1.36 GB
 // read and written) 243 us, of which the copies 223, 6.1 TB/s, 94 % of the copy rate.

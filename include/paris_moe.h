@@ -399,10 +399,11 @@ size_t pmoe_noalloc_scratch_bytes(void);
  * kv_lens[b] - (cu_q[b+1] - t).  Rows behind cu_q[B] belong to no sequence.
  * A table entry outside [0, n_pages) names no page: nothing is read or written
  * through it, and a row that sees such a key gets NaN.  A sequence appears once in a
- * batch (two rows that write one cache place race).  Strides are in elements
- * (positive multiples of 8; the innermost dimension is contiguous).  The reference runs
- * this half through the HF module (Qwen3_5MoeAttention) and its slot-pool cache
- * (engine/runtime/kv_cache.py:220); it has no operator of its own for any of it.
+ * batch (two rows that write one cache place race), and outputs overlap no input.
+ * Strides are in elements (positive multiples of 8; the innermost dimension is
+ * contiguous).  The reference runs this half through the HF module
+ * (Qwen3_5MoeAttention) and its slot-pool cache (engine/runtime/kv_cache.py:220); it has
+ * no operator of its own for any of it.
  *
  * Rotary positions and cache write.  For each row of q and k: the optional
  * per-head RMSNorm (w_qnorm / w_knorm [D], NULL: none; x * rsqrt(mean x^2 + eps) *

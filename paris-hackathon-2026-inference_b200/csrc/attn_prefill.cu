@@ -38,6 +38,7 @@
 // 0.85 PFLOP/s).  Short calls by a block's fixed 7.5 us: 3.5 until the first S, 2.7 from the last
 // product to the end, 1.2 between blocks.
 #include <algorithm>
+#include <cfloat>
 
 #include "paged.cuh"
 #include "pmoe_tc.cuh"
@@ -678,7 +679,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(
       }
       hole = bar_any(1, 256, hole);
     }
-    const float c2 = fabsf(a.scale) * kLog2e;
+    // (never 0, which would make NaN of the -inf that stands for what a row does not see)
+    float c2 = fabsf(a.scale) * kLog2e;
+    if (c2 < FLT_MIN) c2 = FLT_MIN;
     float m = -INFINITY, l = 0.f;  // m in units of S; l relative to m
     // The product P V of tile j has ended.  Tiles alternate between two barriers, and a barrier's
     // parity tells two uses apart: tile j may be asked for only once tile j - 2's product is known

@@ -152,6 +152,33 @@ def check_prefill(new, ctx, Hq, Hkv, D, ps, window=0, sinks=0, seed=0, pad=0, be
     assert not got[sum(new):].any()
 
 
+@pytest.mark.parametrize("scale", [30.0, -2.0, 0.0, 1e-42])
+@pytest.mark.parametrize("D,Hq,new,ctx", [(64, 2, [100, 3], [0, 90]), (128, 4, [5], [2000]),
+                                          (256, 16, [130, 200], [40, 0])])
+def test_prefill_extreme_scales(D, Hq, new, ctx, scale):
+    """One key takes all; all keys weigh the same; also where the keys are split and in pairs."""
+    from paris_moe_b200 import ops
+    pages, table, n = make_cache([a + b for a, b in zip(new, ctx)], 2, D, 16, 3)
+    q, cu = rand_q(sum(new), Hq, D), cu_of(new)
+    got = ops.attn_prefill(q, pages[:, 0, 0], pages[:, 0, 1], table, n, cu, scale, 70, 3)
+    want, bound = R.attention(q, pages[:, 0, 0], pages[:, 0, 1], table, n, cu, scale, 70, 3)
+    R.within(got, want, bound)
+    got = ops.attn_prefill(q, pages[:, 0, 0], pages[:, 0, 1], table, n, cu, scale)
+    want, bound = R.attention(q, pages[:, 0, 0], pages[:, 0, 1], table, n, cu, scale)
+    R.within(got, want, bound)
+
+
+def test_a_scale_that_is_not_a_number_gives_nan_where_keys_are_seen():
+    from paris_moe_b200 import ops
+    pages, table, n = make_cache([40, 0], 2, 64, 16)
+    q = rand_q(2, 4, 64)
+    cu = cu_of([1, 1])
+    k, v = pages[:, 0, 0], pages[:, 0, 1]
+    for got in (ops.attn_decode(q, k, v, table, n, math.nan),
+                ops.attn_prefill(q, k, v, table, n, cu, math.nan)):
+        assert torch.isnan(got[0]).all() and not got[1].any()
+
+
 @pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize("ps", [16, 32, 64, 128])
 def test_prefill_lengths(D, ps):

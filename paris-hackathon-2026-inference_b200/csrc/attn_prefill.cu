@@ -949,16 +949,17 @@ struct Plan {
 int64_t slots_of(int T, int B, int per) { return (int64_t(T) + per - 1) / per + B - 1; }
 // `keys`: the most that a row may see.
 //
-// Split: while the parts still fit on the GPU at once (152 CTAs took 69 us where 114 took 49), and
-// no further than a part's tiles and the join cost the same: a tile takes about 1.2 us, joining
-// one more part 0.4, so sqrt(3 tiles) parts.  64 tokens on 8000 keys, 2 heads of 256: 100 us whole,
-// 26.5 in 13 to 16 parts, 39 in 24; one token on 30000 keys: 338 whole, 37 in 24 parts, 50 in
-// 74.  Below 6 tiles the join costs what it saves (16 x 8 tokens on 600 keys: 17.8 whole, 18.4 in
-// 2; 4 heads of 128: 13.9 and 16.8).
+// Split: while the parts still fit on the GPU at once (300 tokens on 8000 keys: 152 CTAs took 66 us
+// where 114 took 46), and no further than a part's tiles and the join cost the same: a tile takes
+// about 1.2 us, joining one more part 0.4, so sqrt(3 tiles) parts.  64 tokens on 8000 keys, 2
+// heads of 256: 95 us whole, 25 in 13 parts, 37 in 24; one token on 30000 keys: 328 whole, 34 in
+// 24 parts, 47 in 74.  Below 6 tiles the join costs what it saves (16 x 8 tokens on 600 keys: 15.1
+// whole, 15.4 in 2; 4 heads of 128: 11.2 and 14.1).
 //
-// Pairs: at D = 256, where sequences have two CTAs' rows: one prompt of 8192 tokens 400 us, 476
-// in single CTAs; 16 tokens each for 64 sequences 107 and 79.  At D = 128 a lone CTA hides its
-// copies: 2 x 4096 tokens 32/4 heads of 128 took 1 to 8 % longer in pairs.
+// Pairs: at D = 256, where sequences have two CTAs' rows: one prompt of 2048 tokens 39 us, 42 in
+// single CTAs, of 8192 back to back 446 and 462; 16 tokens each for 64 sequences 106 in pairs,
+// 78 in single CTAs.  At D = 128 a lone CTA hides its copies: 2 x 4096 tokens of 32/4 heads of
+// 128 took 1 to 8 % longer in pairs.
 Plan plan_of(int T, int B, int Hq, int Hkv, int D, int64_t keys) {
   const int per = kRows / (Hq / Hkv);
   const int64_t slots = slots_of(T, B, per), rows = (int64_t(T) + per - 1) / per;

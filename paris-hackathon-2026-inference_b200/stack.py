@@ -56,15 +56,15 @@ class MoEStack:
         self.eps = float(eps)
         shape = blocks[0].shape
         self.group = group or EPGroup(shape.E, shape.H, shape.K, mode="fused")
-        self._ws = None
         self._graph = None
 
     def _workspace(self, T: int, device) -> torch.Tensor:
+        """Scratch of one forward.  Each has its own, from the caching allocator's pool of the
+        stream that it runs on, so calls on two streams do not meet; one that is captured
+        gets it from its graph's pool, which lives as long as the graph."""
         s = self.blocks[0].shape
         nbytes = _lib.workspace_size(T, s.H, s.E, s.K, s.I, s.Is)
-        if self._ws is None or self._ws.numel() < nbytes or self._ws.device != device:
-            self._ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        return self._ws
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
     def forward(self, h: torch.Tensor) -> torch.Tensor:
         if h.dtype != _BF16 or not h.is_cuda or not h.is_contiguous():
@@ -79,15 +79,17 @@ class MoEStack:
     def capture(self, h_static: torch.Tensor) -> torch.cuda.CUDAGraph:
         """Capture ``forward(h_static)`` (in place) into a CUDA graph; replay with
         ``graph.replay()`` after writing the step's input into ``h_static``."""
-        self._workspace(h_static.shape[0], h_static.device)
+        return self._capture(h_static)
+
+    def _capture(self, h_static: torch.Tensor, *args) -> torch.cuda.CUDAGraph:
         s = torch.cuda.Stream(device=h_static.device)
         s.wait_stream(torch.cuda.current_stream(h_static.device))
         with torch.cuda.stream(s):   # warm-up outside the graph (lazy init, tensor maps)
-            self.forward(h_static.clone())
+            self.forward(h_static.clone(), *args)
         torch.cuda.current_stream(h_static.device).wait_stream(s)
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
-            self.forward(h_static)
+            self.forward(h_static, *args)
         self._graph = g
         return g
 
@@ -185,17 +187,7 @@ class DecoderStack(MoEStack):
         ``h_static`` and the step's tensors hold then, so the lengths and tables may have moved
         on (captured at the largest table width).  The warm-up runs outside the graph and writes
         the step's keys and values once."""
-        self._workspace(h_static.shape[0], h_static.device)
-        s = torch.cuda.Stream(device=h_static.device)
-        s.wait_stream(torch.cuda.current_stream(h_static.device))
-        with torch.cuda.stream(s):
-            self.forward(h_static.clone(), step)
-        torch.cuda.current_stream(h_static.device).wait_stream(s)
-        g = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(g):
-            self.forward(h_static, step)
-        self._graph = g
-        return g
+        return self._capture(h_static, step)
 
 
 def make_attention_weights(n_layers: int, H: int = W.HIDDEN, heads: int = 16, kv_heads: int = 2,

@@ -66,6 +66,10 @@ class MoEStack:
         nbytes = _lib.workspace_size(T, s.H, s.E, s.K, s.I, s.Is)
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
+    def _held(self):
+        """What a captured forward reads and writes besides its arguments."""
+        return [self.group, self.norms, *(t for b in self.blocks for t in b.tensors())]
+
     def forward(self, h: torch.Tensor) -> torch.Tensor:
         if h.dtype != _BF16 or not h.is_cuda or not h.is_contiguous():
             raise RuntimeError("MoEStack: h must be a contiguous bf16 CUDA tensor")
@@ -78,10 +82,11 @@ class MoEStack:
     # -- CUDA graph of the whole stack at a fixed T ---------------------------
     def capture(self, h_static: torch.Tensor) -> torch.cuda.CUDAGraph:
         """Capture ``forward(h_static)`` (in place) into a CUDA graph; replay with
-        ``graph.replay()`` after writing the step's input into ``h_static``."""
-        return self._capture(h_static)
+        ``graph.replay()`` after writing the step's input into ``h_static``.  The graph keeps
+        what it reads and writes alive."""
+        return self._capture([], h_static)
 
-    def _capture(self, h_static: torch.Tensor, *args) -> torch.cuda.CUDAGraph:
+    def _capture(self, held, h_static: torch.Tensor, *args) -> torch.cuda.CUDAGraph:
         s = torch.cuda.Stream(device=h_static.device)
         s.wait_stream(torch.cuda.current_stream(h_static.device))
         with torch.cuda.stream(s):   # warm-up outside the graph (lazy init, tensor maps)
@@ -90,6 +95,7 @@ class MoEStack:
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
             self.forward(h_static, *args)
+        g.held = [h_static, *held, *self._held()]
         self._graph = g
         return g
 
@@ -186,8 +192,13 @@ class DecoderStack(MoEStack):
         """Capture ``forward(h_static, step)`` into a CUDA graph.  A replay works on what
         ``h_static`` and the step's tensors hold then, so the lengths and tables may have moved
         on (captured at the largest table width).  The warm-up runs outside the graph and writes
-        the step's keys and values once."""
-        return self._capture(h_static, step)
+        the step's keys and values once.  The graph keeps what it reads and writes alive (the
+        step's tensors and the cache's pages among it)."""
+        return self._capture([] if step is None else list(vars(step).values()), h_static, step)
+
+    def _held(self):
+        return [*super()._held(), self.cache.pages, self.inv_freq,
+                *(t for w in self.attention if w is not None for t in vars(w).values())]
 
 
 def make_attention_weights(n_layers: int, H: int = W.HIDDEN, heads: int = 16, kv_heads: int = 2,

@@ -48,6 +48,23 @@ def test_a_longer_call_after_a_capture_leaves_the_graph_its_scratch():
     assert untouched(taken)
 
 
+def test_a_graph_keeps_its_step_alive():
+    """The tensors of a step that the caller has dropped are not given to others."""
+    x = rows(2, 3)
+    st, _ = make()
+    hs = x.clone()
+    graph = st.capture(hs, step_of(st, [0, 3], [1, 1]))
+    hs.copy_(x)
+    taken = occupy()
+    small = [torch.full((n,), 0x5a, dtype=torch.uint8, device=DEV) for n in range(8, 512, 8)]
+    graph.replay()
+    got = hs.clone()
+    other, _ = make()
+    want = other.forward(x.clone(), step_of(other, [0, 3], [1, 1]))
+    assert torch.equal(got, want)
+    assert untouched(taken) and untouched(small)
+
+
 @pytest.mark.parametrize("attention", [False])
 def test_two_graphs_replay_at_once(attention):
     """Two captured steps, of one stack or (with caches of their own) of two, on two streams."""

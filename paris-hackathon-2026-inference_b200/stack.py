@@ -83,7 +83,7 @@ class MoEStack:
     def capture(self, h_static: torch.Tensor) -> torch.cuda.CUDAGraph:
         """Capture ``forward(h_static)`` (in place) into a CUDA graph; replay with
         ``graph.replay()`` after writing the step's input into ``h_static``.  The graph keeps
-        what it reads and writes alive."""
+        what it reads and writes alive and shares no scratch with other calls."""
         return self._capture([], h_static)
 
     def _capture(self, held, h_static: torch.Tensor, *args) -> torch.cuda.CUDAGraph:
@@ -93,8 +93,12 @@ class MoEStack:
             self.forward(h_static.clone(), *args)
         torch.cuda.current_stream(h_static.device).wait_stream(s)
         g = torch.cuda.CUDAGraph()
+        # (torch keeps the matrix products' scratch by stream, and all captures use one stream:
+        # cleared before, it comes from this graph's pool; cleared after, the next has its own)
+        torch._C._cuda_clearCublasWorkspaces()
         with torch.cuda.graph(g):
             self.forward(h_static, *args)
+        torch._C._cuda_clearCublasWorkspaces()
         g.held = [h_static, *held, *self._held()]
         self._graph = g
         return g
@@ -193,7 +197,7 @@ class DecoderStack(MoEStack):
         ``h_static`` and the step's tensors hold then, so the lengths and tables may have moved
         on (captured at the largest table width).  The warm-up runs outside the graph and writes
         the step's keys and values once.  The graph keeps what it reads and writes alive (the
-        step's tensors and the cache's pages among it)."""
+        step's tensors and the cache's pages among it) and shares no scratch with other calls."""
         return self._capture([] if step is None else list(vars(step).values()), h_static, step)
 
     def _held(self):

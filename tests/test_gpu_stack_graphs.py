@@ -65,7 +65,7 @@ def test_a_graph_keeps_its_step_alive():
     assert untouched(taken) and untouched(small)
 
 
-@pytest.mark.parametrize("attention", [False])
+@pytest.mark.parametrize("attention", [False, True])
 def test_two_graphs_replay_at_once(attention):
     """Two captured steps, of one stack or (with caches of their own) of two, on two streams."""
     from paris_moe_b200 import stack
@@ -106,3 +106,21 @@ def test_eager_calls_of_a_stack_on_two_streams_at_once():
     torch.cuda.synchronize()
     for i in (0, 1):
         assert all(torch.equal(y, want[i]) for y in got[i])
+
+
+def test_a_graph_outlives_the_one_captured_before_it():
+    """The second graph's matrix products do not work in the first one's memory."""
+    x = rows(6, 9)
+    st, _ = make()
+    step = step_of(st, list(range(6)), [1] * 6)
+    hs = x.clone()
+    first = st.capture(x.clone(), step)
+    second = st.capture(hs, step)
+    del first
+    st._graph = None
+    torch.cuda.empty_cache()
+    taken = occupy()
+    hs.copy_(x)
+    second.replay()
+    want = st.forward(x.clone(), step)
+    assert torch.equal(hs, want) and untouched(taken)

@@ -478,9 +478,11 @@ int pmoe_pages_grow(int32_t* refs, int n_pages, int page_size, int32_t* tables,
 
 /* fork: empty sequence dst[i] becomes the first keep[i] tokens of src[i]: the full
  * pages are shared (refs + 1), a partly filled last page is copied (its used rows) into
- * a fresh one.  ok[i] = 1, or 0 and nothing changed: an index out of range, dst[i]
+ * a fresh one.  Full pages that the source has given up (free with a window) are missing in the
+ * copy too.  ok[i] = 1, or 0 and nothing changed: an index out of range, dst[i]
  * not empty, named by an earlier request or the source of any request, keep[i] < 0
- * or beyond the source's length, or no page left (as in grow). */
+ * or beyond the source's length, a partly filled last page that the source has given up (the tokens
+ * to come would have no page), or no page left (as in grow). */
 int pmoe_pages_fork(uint16_t* pages, int n_pages, int chunks, int page_size, int D,
                     int32_t* refs, int32_t* tables, int64_t table_stride, int max_pages, int S,
                     int32_t* lens, const int32_t* src, const int32_t* dst, const int32_t* keep,

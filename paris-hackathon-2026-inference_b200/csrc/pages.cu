@@ -183,10 +183,10 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(
     if (s < 0 || s >= p.S || d < 0 || d >= p.S || mark[d] != i || mark[s] != 0x7fffffff || k < 0 ||
         k > int64_t(p.max_pages) << p.page_shift)
       return -1;
-    const int full = k >> p.page_shift;
-    const int tail = k & (ps - 1) ? p.tables[s * p.table_stride + full] : -1;
-    if (p.lens[d] != 0 || k > p.lens[s]) return -1;
-    return int(tail >= 0 && tail < p.n_pages);
+    const bool part = k & (ps - 1);  // the last page is partly filled: it is copied, so it must be there
+    const int tail = part ? p.tables[s * p.table_stride + (k >> p.page_shift)] : 0;
+    if (p.lens[d] != 0 || k > p.lens[s] || (part && (tail < 0 || tail >= p.n_pages))) return -1;
+    return int(part);
   });
   for (int i = tid; i < n; i += kPlanThreads) {
     const bool yes = q.need[i] >= 0 && q.end[i] <= found;

@@ -55,7 +55,9 @@ class PagedKVCache:
                               self._list(add), self.page_size)
 
     def fork(self, src, dst, keep=None) -> torch.Tensor:
-        """Empty sequences ``dst`` become the first ``keep`` tokens (default: all) of ``src``."""
+        """Empty sequences ``dst`` become the first ``keep`` tokens (default: all) of ``src``.  Refused
+        (ok 0) among others where ``keep`` ends inside a page that ``src`` has given up behind a
+        window."""
         src = self._list(src)
         if keep is None:   # (the call itself refuses sources out of range)
             keep = self.lens[src.clamp(0, self.lens.shape[0] - 1)]

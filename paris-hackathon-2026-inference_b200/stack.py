@@ -163,7 +163,7 @@ class DecoderStack(MoEStack):
         T, Hq, Hkv, D = h.shape[0], w.heads, w.kv_heads, w.head_dim
         qkv = ops.rmsnorm(h, w.w_norm, self.eps) @ w.w_qkv.t()
         q, k, v = qkv.split([qkv.shape[1] - 2 * Hkv * D, Hkv * D, Hkv * D], 1)
-        q = q.view(T, Hq, -1)
+        q = q.view(T, Hq, (2 if w.gated else 1) * D)
         cache = (self.cache.k(layer), self.cache.v(layer), step.page_table, step.kv_lens)
         r = ops.rope_append(q[..., :D], k.view(T, Hkv, D), v.view(T, Hkv, D), step.positions,
                             self.inv_freq, self.sections, self.interleaved, *cache,

@@ -100,3 +100,18 @@ def test_each_layer_writes_and_reads_its_own_part_of_the_cache(gated, window, si
             want = layer.expected_pages(at).view(torch.int16)
             for s in (st, twin):
                 assert torch.equal(s.cache.pages[:, at].cpu().view(torch.int16), want)
+
+
+@pytest.mark.parametrize("single", [False, True])
+def test_a_step_without_tokens(single):
+    from paris_moe_b200 import Step
+    st, _ = make()
+    step_of(st, [0], [5])
+    i32 = dict(dtype=torch.int32, device=DEV)
+    rows = torch.tensor([], dtype=torch.int64, device=DEV) if single else torch.tensor([0], device=DEV)
+    step = Step(st.cache.tables[rows], st.cache.lens[rows], torch.zeros((3, 0), dtype=torch.int64, device=DEV),
+                None if single else torch.zeros(2, **i32))
+    before = st.cache.pages.clone()
+    h = torch.empty((0, H), dtype=R.BF16, device=DEV)
+    out = st.forward(h, step)
+    assert out.shape == (0, H) and torch.equal(st.cache.pages, before)

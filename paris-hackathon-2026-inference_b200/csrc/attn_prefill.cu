@@ -253,14 +253,15 @@ __device__ __forceinline__ bool find_tile(const AttnArgs& a, int per, int x, Til
   const int32_t* cu = a.cu_q;
   const int lo = last_at_or_before(a.kv.B, x, [=](int b) { return cu[b] / per + b; });
   if (lo < 0) return false;
-  const int c0 = a.cu_q[lo], c1 = min(a.cu_q[lo + 1], a.T), len = a.kv.kv_lens[lo];
+  // (cu_q may count rows that the call does not have)
+  const int c0 = a.cu_q[lo], end = a.cu_q[lo + 1], c1 = min(end, a.T), len = a.kv.kv_lens[lo];
   const int i = x - (c0 / per + lo);
   if (c0 < 0 || c1 <= c0 || i < 0 || i > (c1 - c0 - 1) / per) return false;
   o->b = lo;
   o->t0 = c0 + i * per;
   o->n = min(per, c1 - o->t0);
   o->len = kv_len_of(len, a.kv.max_pages, a.kv.page_shift, &o->over);
-  o->p0 = o->len - (c1 - o->t0);
+  o->p0 = o->len - (end - o->t0);
   return true;
 }
 

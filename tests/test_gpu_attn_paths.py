@@ -48,3 +48,17 @@ def test_bookkeeping_of_more_sequences_than_marks_in_shared_memory():
     p.check()
     p.grow(slots[4400:] + [0, S, -1], [20] * 603)
     p.check()
+
+
+@pytest.mark.parametrize("D,Hq,T", [(64, 4, 100), (128, 2, 3), (256, 16, 259), (256, 16, 300), (64, 16, 1)])
+def test_prefill_of_the_first_rows_of_a_batch(D, Hq, T):
+    """cu_q may count more rows than the call has: a row's index goes by its sequence's own tokens."""
+    from paris_moe_b200 import ops
+    new, ctx = [90, 0, 170, 41], [700, 3, 0, 12]
+    pages, table, n = make_cache([a + b for a, b in zip(new, ctx)], 2 if Hq < 16 else 1, D, 16)
+    q, cu = rand_q(sum(new), Hq, D), cu_of(new)
+    k, v = pages[:, 0, 0], pages[:, 0, 1]
+    for window, sinks in ((0, 0), (40, 3)):
+        want, bound = R.attention(q, k, v, table, n, cu, 0.1, window, sinks)
+        got = ops.attn_prefill(q[:T], k, v, table, n, cu, 0.1, window, sinks)
+        R.within(got, want[:T], bound[:T], f"{T} of {sum(new)} rows")

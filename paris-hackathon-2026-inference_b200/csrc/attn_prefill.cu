@@ -398,7 +398,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(
   const uint32_t tm_o = __shfl_sync(0xffffffffu, s_tmem, 0), tm_p = tm_o + D, tm_s = tm_p + 128;
 
   if (warp >= 12) {
-    // ---- V of the cut tiles: a thread has 64 dims of a key of each chunk
+    // ---- V of the cut tiles: a thread has 64 dims of a key of each chunk.  A wait that runs out in
+    // one warp stops all four, at the barrier that they next meet at: a warp that left by itself
+    // would keep the others there.
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsClean));
     const int line = tid & 127, row = line % C::kVr, wc = warp & 3;
     const int of = rank * C::kVg + wc * 32 / C::kVr;  // 64 dims of D
@@ -411,7 +413,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(
       for (int c = 0; c < C::kVc; ++c) {
         const int u = e * C::kVc + c;
         // (one warp polls: four took issue slots from the softmax warps)
-        if (wc == 0) ok = warp_wait(&cut_full[u % kCuts], (u / kCuts) & 1);
+        if (wc == 0) ok = ok && warp_wait(&cut_full[u % kCuts], (u / kCuts) & 1);
         ok = !bar_any(6, 128, !ok);
         if (!ok) break;
         const int jj = k0 + c * C::kVr + row;
@@ -500,8 +502,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefill_kernel(
         tc_fence_before();
         __syncwarp();
       }
-      if (!ok) break;
-      if (lane == 0)
+      if (ok && lane == 0)
         for (int c = 0; c < C::kVc; ++c) {
           uint64_t* bar = &v_full[(j * C::kVc + c) % C::kSlots];
           if (PAIR)

@@ -464,6 +464,10 @@ int pmoe_attn_prefill(const uint16_t* q, int64_t q_stride_t, int64_t q_stride_h,
  * order without a host sync, can be captured, and are deterministic: free pages are
  * handed out lowest number first, requests served in list order.  workspace:
  * pmoe_pages_workspace bytes, contents irrelevant before and after.
+ * Only these calls change refs, tables and lens.  Lengths only grow: to take tokens back (rejected
+ * drafts), fork those that stay into an empty sequence and free the old one.  (A length lowered by
+ * hand loses the pages behind it, whose table entries grow overwrites, and lets new tokens into
+ * pages that others share.)
  *
  * grow: sequence slots[i] gets add[i] more tokens and the pages they need.  ok[i] =
  * 1, or 0 and nothing changed: a slot out of range, add < 0, a length beyond the

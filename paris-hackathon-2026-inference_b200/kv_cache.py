@@ -7,6 +7,10 @@ page; 0: free), ``tables [max_seqs, max_pages]`` (-1: no page) and ``lens [max_s
 The reference keeps one slot of fixed length per sequence instead
 (engine/runtime/kv_cache.py:220).
 
+Only the calls change these.  Lengths only grow: tokens are taken back (rejected drafts) by
+``fork`` of those that stay into an empty slot and ``free`` of the old one; a length lowered by
+hand would lose the pages behind it and let new tokens into pages that branches share.
+
 The calls run in stream order without a host sync and can be captured in CUDA graphs when
 their lists are device tensors.  ``grow`` and ``fork`` return ``ok`` (int32, one per
 request; 0: refused, nothing changed) on the device.

@@ -1,4 +1,4 @@
-"""Page bookkeeping of sequences that have given pages up behind a window."""
+"""Page bookkeeping of sequences that have given pages up behind a window, and of rejected drafts."""
 from __future__ import annotations
 
 import pytest
@@ -59,3 +59,26 @@ def test_a_fork_whose_last_page_is_not_in_the_pool_is_refused():
         c.free([2])
     c.tables[0, 2] = last
     assert c.fork([0], [1]).tolist() == [1]
+
+
+def test_rejected_drafts_are_given_back_by_forking_what_stays():
+    """Lengths only grow; a sequence is shortened by forking the tokens that stay into an empty slot
+    and freeing the old one.  No page is lost, and the keys that stay are the same."""
+    from paris_moe_b200 import PagedKVCache
+    g = torch.Generator().manual_seed(1)
+    c = PagedKVCache(40, 16, 2, 1, 64, 4, 160)
+    c.pages.copy_(torch.randn(c.pages.shape, generator=g))
+    one = lambda s, n: c.k(1)[c.tables[s, :-(-n // 16)].long(), 0].reshape(-1, 64)[:n].clone()  # noqa: E731
+    slot, spare, n = 0, 1, 30
+    assert c.grow([slot], [n]).tolist() == [1]
+    for accepted in (0, 1, 2, 5, 5, 3, 0, 4):
+        assert c.grow([slot], [5]).tolist() == [1]            # five drafted tokens
+        kept = one(slot, n + accepted)
+        if accepted < 5:
+            assert c.fork([slot], [spare], [n + accepted]).tolist() == [1]
+            c.free([slot])
+            slot, spare = spare, slot
+        n += accepted
+        assert int(c.lens[slot]) == n and torch.equal(one(slot, n), kept)
+        assert int((c.refs > 0).sum()) == -(-n // 16)
+        consistent(c)

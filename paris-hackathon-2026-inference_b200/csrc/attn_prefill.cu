@@ -29,14 +29,15 @@
 // 0 x inf is NaN: in tiles that are cut by some row's sight, V rows that nobody sees or that
 // hold a non-finite number are zeroed in shared memory, and the latter are added to the rows
 // that see them one by one.  Warps of their own do this as the tile lands: in the softmax warps it
-// cost 2 x 4096 tokens of 32/4 heads of 128 260 us instead of 224 (215 with no cleaning at all).
+// cost prompts of 4096 and 2531 tokens, 32/4 heads of 128, 260 us instead of 224 (215 with no
+// cleaning at all).
 //
-// Bound by the tensor cores for long prompts at D = 256: 8192 tokens of 16/2 heads 390 us (550
-// GFLOP, 1.41 PFLOP/s, 82 % of a matrix product's best; under the power cap of a long run 447), a
-// tile of a pair 2100 cycles where the products alone need 2048.  At D = 128 and 64 by a row's softmax:
-// 2000 cycles a tile and group, 1024 of them the exponential unit (224 us for the 2 x 4096 above,
-// 0.85 PFLOP/s).  Short calls by a block's fixed 7.5 us: 3.5 until the first S, 2.7 from the last
-// product to the end, 1.2 between blocks.
+// Bound by the tensor cores for long prompts at D = 256: 8192 tokens of 16/2 heads 383 us, 20
+// calls in a graph (550 GFLOP, 1.43 PFLOP/s, 83 % of a matrix product's best; under the power cap
+// of a long run 447), a tile of a pair 2100 cycles where the products alone need 2048.  At D = 128
+// and 64 by a row's softmax: 2000 cycles a tile and group, 1024 of them the exponential unit (219 us
+// for the 4096 and 2531 tokens above, 0.87 PFLOP/s; 203 at D = 64).  Short calls by a block's fixed
+// 7.5 us: 3.5 until the first S, 2.7 from the last product to the end, 1.2 between blocks.
 #include <algorithm>
 #include <cfloat>
 
@@ -949,19 +950,24 @@ struct Plan {
 };
 // Slots that find_tile uses: floor(cu / per) + ceil(n / per) <= ceil((cu + n) / per).
 int64_t slots_of(int T, int B, int per) { return (int64_t(T) + per - 1) / per + B - 1; }
-// `keys`: the most that a row may see.
+// `keys`: the most that a row may see, by the table's width and the window.  (The lengths are on
+// the device.  A table is as wide as its cache's longest sequence may get, so that few rows on few
+// keys take parts that hold nothing: their CTAs set up and leave, and the join walks them.  On
+// a table 32768 tokens wide 64 new tokens took 14.5 us, on one as wide as they are 10.7; 64 on
+// 836 keys 16.6 and 15.6; 300 new 15.0 and 12.9; 64 on 30000 keys, and 32 prompts, the same.)
 //
 // Split: while the parts still fit on the GPU at once (300 tokens on 8000 keys: 152 CTAs took 66 us
 // where 114 took 46), and no further than a part's tiles and the join cost the same: a tile takes
 // about 1.2 us, joining one more part 0.4, so sqrt(3 tiles) parts.  64 tokens on 8000 keys, 2
 // heads of 256: 95 us whole, 25 in 13 parts, 37 in 24; one token on 30000 keys: 328 whole, 34 in
-// 24 parts, 47 in 74.  Below 6 tiles the join costs what it saves (16 x 8 tokens on 600 keys: 15.1
-// whole, 15.4 in 2; 4 heads of 128: 11.2 and 14.1).
+// 24 parts, 47 in 74.  Below 6 tiles the join costs what it saves (16 times up to 8 tokens on up
+// to 600 keys: 15.1 whole, 15.4 in 2; 4 heads of 128: 11.2 and 14.1).  All on tables as wide as
+// the longest sequence.
 //
 // Pairs: at D = 256, where sequences have two CTAs' rows: one prompt of 2048 tokens 39 us, 42 in
-// single CTAs, of 8192 back to back 446 and 462; 16 tokens each for 64 sequences 106 in pairs,
-// 78 in single CTAs.  At D = 128 a lone CTA hides its copies: 2 x 4096 tokens of 32/4 heads of
-// 128 took 1 to 8 % longer in pairs.
+// single CTAs, of 8192 back to back 446 and 462; up to 16 tokens each for 64 sequences on up to
+// 4000 keys 106 in pairs, 78 in single CTAs.  At D = 128 a lone CTA hides its copies: 4096 and 2531
+// tokens of 32/4 heads of 128 took 1 to 8 % longer in pairs.
 Plan plan_of(int T, int B, int Hq, int Hkv, int D, int64_t keys) {
   const int per = kRows / (Hq / Hkv);
   const int64_t slots = slots_of(T, B, per), rows = (int64_t(T) + per - 1) / per;

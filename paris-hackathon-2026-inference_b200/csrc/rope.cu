@@ -29,7 +29,7 @@ __device__ __forceinline__ int rope_axis(const RopeArgs& a, int i) {
 // were loaded.  A batch of rows is on its way while the angles are worked out.
 //
 // 8192 tokens of 16 + 2 heads of 256 (168 MB): 34.5 us, 4.9 TB/s, 75 % of the copy rate.  Bound by
-// instructions (128 a row, 61 % of the issue slots): the first version took 320 a row and
+// instructions (128 a row, 63 % of the issue slots): the first version took 320 a row and
 // 76 us, one with the factors in shared memory 51, this one with batches of 4 rows (110
 // registers, half the warps) 44.  64 tokens, eight warps each: 4.5 us, a chain of latencies.
 constexpr int kBatch = 2;  // row slots a warp holds at a time, and as many on their way

@@ -139,7 +139,8 @@ class Step:
 class DecoderStack(MoEStack):
     """Decoder layers over a paged cache.  ``attention[l]`` is the layer's attention half, or None
     for a layer whose token mixing happens elsewhere; the k-th layer that has one uses layer k of
-    ``cache``.  ``forward(h, step)`` updates the [T, H] residual stream ``h`` in place."""
+    ``cache``.  ``forward(h, step)`` updates the [T, H] residual stream ``h`` in place.
+    Across ranks T is at most the group's ``t_max`` (its decode exchange)."""
 
     def __init__(self, norms: torch.Tensor, blocks, attention, cache, inv_freq: torch.Tensor,
                  sections, interleaved: bool = True, window: int = 0, sinks: int = 0,
@@ -182,6 +183,9 @@ class DecoderStack(MoEStack):
             raise RuntimeError("DecoderStack: h must be a contiguous bf16 CUDA tensor")
         if step is None and any(w is not None for w in self.attention):
             raise RuntimeError("DecoderStack: attention layers need a Step")
+        if self.group.world > 1 and not self.group.uses_exchange(h.shape[0]):
+            # (what layer_forward would say behind the first attention half)
+            raise ValueError("DecoderStack across ranks needs the fused exchange (T <= t_max)")
         ws = self._workspace(h.shape[0], h.device)
         layer = 0
         for l, b in enumerate(self.blocks):

@@ -115,3 +115,20 @@ def test_a_step_without_tokens(single):
     h = torch.empty((0, H), dtype=R.BF16, device=DEV)
     out = st.forward(h, step)
     assert out.shape == (0, H) and torch.equal(st.cache.pages, before)
+
+
+def test_a_step_too_long_for_the_exchange_is_refused_before_it_changes_anything():
+    """Across ranks a layer takes as many tokens as the exchange holds: more are refused ahead of the
+    first layer's attention half, not behind it."""
+    from paris_moe_b200 import stack
+    from paris_moe_b200.ep import EPGroup
+    one, att = make()
+    group = EPGroup.emulated(16, H, 4, rank=0, world=2)          # no exchange buffers at all
+    st = stack.DecoderStack(one.norms, one.blocks, att, one.cache, one.inv_freq, SECTIONS, group=group)
+    step = step_of(st, [0, 2], [30, 40])
+    h = torch.randn(70, H, generator=torch.Generator().manual_seed(1)).to(R.BF16).to(DEV)
+    before, pages = h.clone(), st.cache.pages.clone()
+    with pytest.raises(ValueError, match="fused exchange"):
+        st.forward(h, step)
+    assert torch.equal(h, before) and torch.equal(st.cache.pages, pages)
+    group.close()
